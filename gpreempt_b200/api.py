@@ -298,6 +298,122 @@ def gemm_tiles(m: int, n: int) -> int:
     return t.value
 
 
+# ---- serving a decoder -------------------------------------------------------------------------
+
+
+def _address(x) -> int | None:
+    """Device address of a DeviceBuffer, an array with data_ptr() or an integer; None stays None."""
+    if x is None or isinstance(x, int):
+        return x
+    if hasattr(x, "data_ptr"):
+        return x.data_ptr()
+    return x.ptr.value
+
+
+class LmContext(_Resettable):
+    """Scratch memory of kv_append, kv_attend and token_scores (arrival counters and partial results).  Launches
+    that share one run in one stream or are ordered by events."""
+
+    def __init__(self):
+        super().__init__()
+        n = ctypes.c_size_t()
+        check(B.load().gpx_lm_ctx_bytes(ctypes.byref(n)))
+        self._buf = DeviceBuffer(n.value)
+        self.reset()
+
+    def reset(self) -> None:
+        self._enqueue_reset(B.load().gpx_lm_ctx_reset)
+
+    def status(self) -> tuple[int, int]:
+        """(code, where) of the first launch since the reset that met something wrong on the device; (0, 0) = none."""
+        err, where = ctypes.c_int(), ctypes.c_int()
+        check(B.load().gpx_lm_status(self.buf.ptr, ctypes.byref(err), ctypes.byref(where)))
+        return err.value, where.value
+
+
+class KvCache:
+    """A pool of pages of 8-bit keys and values with a scale for each page and head.  Without arrays of the caller
+    it allocates its own (zeroed)."""
+
+    def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, k=None, v=None, k_scale=None, v_scale=None):
+        self.pages, self.page_tokens, self.kv_heads, self.head_dim = pages, page_tokens, kv_heads, head_dim
+        self.handle = ctypes.c_void_p()
+        self._own = []
+        if k is None:
+            for n in (pages * kv_heads * page_tokens * head_dim,) * 2 + (pages * kv_heads * 4,) * 2:
+                self._own.append(DeviceBuffer(n))
+                self._own[-1].zero()
+            k, v, k_scale, v_scale = self._own
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        check(B.load().gpx_kv_cache_create(_address(k), _address(v), _address(k_scale), _address(v_scale), pages, page_tokens, kv_heads,
+                                           head_dim, ctypes.byref(self.handle)))
+
+    def free(self) -> None:
+        if self.handle:
+            B.load().gpx_kv_cache_destroy(self.handle)
+            self.handle = ctypes.c_void_p()
+        for b in self._own:
+            b.free()
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class KvBatch:
+    """One step's ragged batch: int32 arrays on the device with the sequences' page numbers [seqs][table_ld], their
+    lengths (new tokens among them) and the offsets of their new tokens [seqs + 1]."""
+
+    def __init__(self, seqs: int, tokens: int, most_new: int, table, context, first, table_ld: int):
+        self.arrays = (table, context, first)
+        self.struct = B.KvBatch(_address(table), _address(context), _address(first), table_ld, seqs, tokens, most_new)
+        self._ref = ctypes.byref(self.struct)
+
+
+class Rope:
+    """Position rotation of the first `rotated` elements of a head: float tables [positions][rotated / 2], pairs of
+    elements j and j + rotated / 2, or 2 j and 2 j + 1 if `paired`."""
+
+    def __init__(self, cos, sin, positions: int, rotated: int, paired: bool = False):
+        self.arrays = (cos, sin)
+        self.cos, self.sin, self.positions, self.rotated, self.paired = _address(cos), _address(sin), positions, rotated, int(paired)
+
+
+def kv_append(cache: KvCache, batch: KvBatch, q, k, v, q_out, heads: int, dtype: str, ctx: LmContext, rope: Rope | None = None,
+              blp: BlpContext | None = None, stream=None, q_ld: int = 0, k_ld: int = 0, v_ld: int = 0, q_out_ld: int = 0) -> None:
+    """Appends a step's keys and values to the cache; turns queries (q to q_out, or both None) and keys on the way."""
+    h = _h(stream)
+    ctx.order(h)
+    turn = (rope.cos, rope.sin, rope.rotated, rope.positions, rope.paired) if rope is not None else (None, None, 0, 0, 0)
+    args = B.KvAppendArgs(_address(q), _address(k), _address(v), _address(q_out), turn[0], turn[1], q_ld, k_ld, v_ld, q_out_ld, heads,
+                          turn[2], turn[3], turn[4], dtype.encode())
+    check(B.load().gpx_kv_append(cache.handle, batch._ref, ctypes.byref(args), ctx._buf.ptr, _blp_for(blp, h), h))
+
+
+def kv_attend(cache: KvCache, batch: KvBatch, q, out, heads: int, dtype: str, ctx: LmContext, scale: float = 0.0, causal: bool = True,
+              window: int = 0, lse=None, blp: BlpContext | None = None, stream=None, q_ld: int = 0, out_ld: int = 0) -> None:
+    """Attention of a step's new tokens over their sequences' pages (scale 0: 1 / sqrt(head_dim))."""
+    h = _h(stream)
+    ctx.order(h)
+    args = B.KvAttendArgs(_address(q), _address(out), _address(lse), q_ld, out_ld, heads, int(causal), window, scale, dtype.encode())
+    check(B.load().gpx_kv_attend(cache.handle, batch._ref, ctypes.byref(args), ctx._buf.ptr, _blp_for(blp, h), h))
+
+
+def token_scores(logits, rows: int, vocab: int, dtype: str, ctx: LmContext, targets=None, logprob=None, entropy=None, lse=None,
+                 top: int = 0, top_ids=None, top_logprob=None, temperature: float = 1.0, ld: int = 0, blp: BlpContext | None = None,
+                 stream=None) -> None:
+    """Log probabilities of `targets`, entropies and the `top` most likely tokens of each row of logits."""
+    h = _h(stream)
+    ctx.order(h)
+    if not top:  # (arrays of no elements have no address worth passing)
+        top_ids = top_logprob = None
+    args = B.TokenScoresArgs(_address(logits), _address(targets), _address(logprob), _address(entropy), _address(lse), _address(top_ids),
+                             _address(top_logprob), ld, rows, vocab, top, 1.0 / temperature if temperature else 0.0, dtype.encode())
+    check(B.load().gpx_token_scores(ctypes.byref(args), ctx._buf.ptr, _blp_for(blp, h), h))
+
+
 def synth_normal(n: int, seed: int, stream: int = 0, mean: float = 0.0, std: float = 1.0):
     out = np.empty(n, np.float32)
     check(B.load().gpx_synth_normal(out.ctypes.data_as(ctypes.c_void_p), n, seed, stream, mean, std))

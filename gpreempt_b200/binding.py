@@ -49,6 +49,42 @@ class ModelOpts(ctypes.Structure):
     _fields_ = [("batch", ctypes.c_int), ("dtype", ctypes.c_char_p), ("seq_len", ctypes.c_int)]
 
 
+class KvBatch(ctypes.Structure):
+    _fields_ = [
+        ("table", ctypes.c_void_p), ("context", ctypes.c_void_p), ("first", ctypes.c_void_p),
+        ("table_ld", ctypes.c_int), ("seqs", ctypes.c_int), ("tokens", ctypes.c_int), ("most_new", ctypes.c_int),
+    ]
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+        ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+        ("q_ld", ctypes.c_longlong), ("k_ld", ctypes.c_longlong), ("v_ld", ctypes.c_longlong), ("q_out_ld", ctypes.c_longlong),
+        ("heads", ctypes.c_int), ("rotated", ctypes.c_int), ("positions", ctypes.c_int), ("paired", ctypes.c_int),
+        ("dtype", ctypes.c_char_p),
+    ]
+
+
+class KvAttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("q_ld", ctypes.c_longlong), ("out_ld", ctypes.c_longlong),
+        ("heads", ctypes.c_int), ("causal", ctypes.c_int), ("window", ctypes.c_int), ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_char_p),
+    ]
+
+
+class TokenScoresArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p), ("targets", ctypes.c_void_p),
+        ("logprob", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("top_ids", ctypes.c_void_p), ("top_logprob", ctypes.c_void_p),
+        ("ld", ctypes.c_longlong), ("rows", ctypes.c_int), ("vocab", ctypes.c_int), ("top", ctypes.c_int),
+        ("inv_temperature", ctypes.c_float), ("dtype", ctypes.c_char_p),
+    ]
+
+
 def declared_symbols() -> list[str]:
     """Names of all functions include/gpx.h declares."""
     with open(HEADER) as fp:
@@ -111,6 +147,14 @@ _SIGS = {
                                P(MicrobenchSummary)],
     "gpx_fill_uniform": [vp, sz, ci, u64, u64, ctypes.c_float, ctypes.c_float, vp],
     "gpx_count_diff": [vp, vp, sz, P(u64), vp],
+    "gpx_lm_ctx_bytes": [P(sz)],
+    "gpx_lm_ctx_reset": [vp, P(vp)],
+    "gpx_lm_status": [vp, P(ci), P(ci)],
+    "gpx_kv_cache_create": [vp, vp, vp, vp, ci, ci, ci, ci, P(vp)],
+    "gpx_kv_cache_destroy": [vp],
+    "gpx_kv_append": [vp, P(KvBatch), P(KvAppendArgs), vp, P(Blp), vp],
+    "gpx_kv_attend": [vp, P(KvBatch), P(KvAttendArgs), vp, P(Blp), vp],
+    "gpx_token_scores": [P(TokenScoresArgs), vp, P(Blp), vp],
     "gpx_synth_normal": [vp, sz, u64, u64, ctypes.c_float, ctypes.c_float],
     "gpx_synth_uniform": [vp, sz, u64, u64, ctypes.c_float, ctypes.c_float],
     "gpx_model_open": [ctypes.c_char_p, P(ModelOpts), P(vp)],

@@ -1,0 +1,164 @@
+// What the operators of a decoder's serving step share: the paged cache, the description of a ragged batch, the
+// scratch context, and the search for a tile's sequence.
+#pragma once
+
+#include "blp.cuh"
+#include "common.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+struct gpx_kv_cache {
+    unsigned char *k, *v;      // e4m3 codes [page][kv head][slot][element]
+    float *k_scale, *v_scale;  // [page][kv head]
+    int pages, page_tokens, kv_heads, dim;
+    CUtensorMap map_k, map_v;  // rows of `dim` bytes, boxes of min(page_tokens, 64) rows, swizzled
+};
+
+namespace gpx {
+
+// ---- scratch context ------------------------------------------------------------------------------
+
+// Header, arrival counters (zero between launches: whoever joins the parts of a result puts its counter back), and
+// the parts of results that several CTAs share.
+constexpr int kLmCounters = 8192;
+constexpr size_t kLmPartsOffset = 256 + kLmCounters * sizeof(int);
+constexpr size_t kLmPartsBytes = (size_t)64 << 20;
+constexpr size_t kLmCtxBytes = kLmPartsOffset + kLmPartsBytes;
+
+enum LmError {
+    LM_BAD_SPAN = 1,      // first[] / context[] of a sequence contradict each other or the limits given
+    LM_BAD_PAGE = 2,      // a page number outside the cache
+    LM_BAD_POSITION = 3,  // a position past the rotation table
+    LM_GAVE_UP = 4,       // a bounded wait ran out
+    LM_TOO_LONG = 5,      // more blocks of work than 31 bits count
+};
+
+struct LmCtx {
+    int *error;  // {code, sequence or CTA}
+    int *counters;
+    float *parts;
+};
+
+inline LmCtx lm_ctx(void *ctx) {
+    unsigned char *p = static_cast<unsigned char *>(ctx);
+    return {reinterpret_cast<int *>(p), reinterpret_cast<int *>(p + 256), reinterpret_cast<float *>(p + kLmPartsOffset)};
+}
+
+// ---- batch ----------------------------------------------------------------------------------------
+
+constexpr int kLmMaxSeqs = 4096;
+
+struct LmBatch {
+    const int *table;    // [seqs][table_ld] page numbers
+    const int *context;  // [seqs] tokens of a sequence, the new ones among them
+    const int *first;    // [seqs + 1] offsets of the sequences' new tokens
+    int table_ld, seqs, tokens, most_new;
+};
+
+int lm_check_batch(const gpx_kv_batch *b, LmBatch *out);
+int lm_check_blp(const gpx_blp *blp, BlpArgs *out);
+int lm_elem(const char *dtype, bool f32_too, int *elem);  // dtype name -> GPX_LM_*
+
+enum { LM_F32 = 0, LM_BF16 = 1, LM_F16 = 2 };
+
+#if defined(__CUDACC__)
+
+// CTAs of a kernel an SM holds, asked for once a thread, device and size of shared memory (the question costs more
+// than a small launch).
+cudaError_t lm_resident(const void *kernel, int threads, size_t smem, int device, int *per_sm);
+
+__device__ __forceinline__ void lm_fail(int *error, int code, int where) {
+    if (atomicCAS(error, 0, code) == 0) error[1] = where;
+}
+
+struct LmSpan {
+    int first, n, context;  // new tokens [first, first + n) of a sequence of `context` tokens
+};
+
+// A span that contradicts itself or the limits of the batch counts as empty, and is reported.
+__device__ __forceinline__ LmSpan lm_span(const LmBatch &b, int s, int page_tokens, bool new_in_context, int *error) {
+    const int f = b.first[s], e = b.first[s + 1], c = b.context[s];
+    const bool fine = f >= 0 && e >= f && e <= b.tokens && e - f <= b.most_new && c >= 0 &&
+                      c <= (long long)b.table_ld * page_tokens && (!new_in_context || c >= e - f);
+    if (!fine) {
+        lm_fail(error, LM_BAD_SPAN, s);
+        return {0, 0, 0};
+    }
+    return {f, e - f, c};
+}
+
+// prefix[s] = sum of count(0 .. s-1), prefix[seqs] = the total, for all threads of the CTA together.  More than
+// 31 bits of them are reported, and nothing is to be done.
+template <typename F>
+__device__ __forceinline__ int lm_prefix(int *prefix, int seqs, int *error, F &&count) {
+    __shared__ int s_sums[32];
+    __shared__ long long s_carry;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+    if (threadIdx.x == 0) s_carry = 0;
+    for (int s0 = 0; s0 < seqs; s0 += blockDim.x) {
+        const int s = s0 + threadIdx.x;
+        const int own = s < seqs ? count(s) : 0;
+        int sum = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += up;
+        }
+        if (lane == 31) s_sums[wid] = sum;
+        __syncthreads();
+        long long before = s_carry, all = 0;
+        for (int w = 0; w < warps; ++w) {
+            if (w < wid) before += s_sums[w];
+            all += s_sums[w];
+        }
+        if (s < seqs) prefix[s] = (int)(before + sum - own);
+        __syncthreads();
+        if (threadIdx.x == 0) s_carry += all;
+    }
+    __syncthreads();
+    const long long total = s_carry;
+    if (total > 0x7fffffff) {
+        if (threadIdx.x == 0) lm_fail(error, LM_TOO_LONG, 0);
+        return 0;
+    }
+    if (threadIdx.x == 0) prefix[seqs] = (int)total;
+    __syncthreads();
+    return (int)total;
+}
+
+// The sequence whose share of [0, prefix[seqs]) holds i.
+__device__ __forceinline__ int lm_find(const int *prefix, int seqs, int i) {
+    int lo = 0, hi = seqs;  // prefix[lo] <= i < prefix[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= i) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// 2^x, the hardware approximation (relative error ~2^-22; -inf gives 0).
+__device__ __forceinline__ float lm_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two e4m3 codes (the lower byte is the lower element) as a pair of halves: exact.
+__device__ __forceinline__ unsigned e4m3x2_to_f16x2(unsigned short codes) {
+    unsigned d;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(codes));
+    return d;
+}
+
+// Rounded to nearest even; beyond 448 the largest code, NaN stays NaN.
+__device__ __forceinline__ unsigned e4m3x2(float lower, float upper) {
+    unsigned short d;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(upper), "f"(lower));
+    return d;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace gpx

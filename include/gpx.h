@@ -232,6 +232,105 @@ int gpx_fill_uniform(void *dptr, size_t n, int is_bf16, uint64_t seed, uint64_t 
                      float hi, gpx_stream s);
 int gpx_count_diff(const void *a, const void *b, size_t bytes, uint64_t *diff, gpx_stream s);
 
+/* ---- serving a decoder ---------------------------------------------------------------- */
+
+/* Have no counterpart in the reference: the step with which a decoder answers, for latency-critical and
+ * best-effort tenants that bring their own projections (gpx_gemm_bf16).  New keys and values go into a paged cache
+ * of 8-bit codes (gpx_kv_append), the new tokens attend over it (gpx_kv_attend), and the logits are turned into log
+ * probabilities, entropies and alternatives (gpx_token_scores).  All three take a gpx_blp as the kernels above do:
+ * with a preempt word they claim tiles, drain at a tile boundary once it is raised and, launched again with the same
+ * arguments, the same context and the same cursor, go on exactly there.  They allocate nothing and wait for nothing.
+ *
+ * `ctx` is gpx_lm_ctx_bytes() bytes of device memory, 256-byte aligned and zeroed before the first launch; all three
+ * take the same one.  Launches that share a context run in one stream or are ordered by events; what was preempted
+ * is resumed before another operator is given its context, or the context is reset (gpx_lm_ctx_reset, asynchronous,
+ * with *ready as in gpx_blp_ctx_reset).  gpx_lm_status (blocking) reads its error word: 0, or the first of
+ *   1  first[] or context[] of sequence *where contradict each other or the limits given (it was left out),
+ *   2  a page number outside the cache (sequence *where),
+ *   3  a position past the rotation table (sequence *where; its new tokens were left out),
+ *   4  a bounded wait gave up (CTA *where; the results are incomplete),
+ *   5  more work than one launch counts (2^31 - 1 blocks of 64 keys); nothing was done. */
+int gpx_lm_ctx_bytes(size_t *bytes);
+int gpx_lm_ctx_reset(void *ctx, gpx_event *ready);
+int gpx_lm_status(const void *ctx, int *error, int *where);
+
+/* A pool of `pages` pages in the caller's memory.  k and v hold OCP e4m3 codes [page][kv_head][page_tokens][head_dim]
+ * (16-byte aligned); k_scale and v_scale [page][kv_head] are positive floats: an element is code x scale of its page
+ * and head.  page_tokens is 16, 32, 64 or 128; head_dim 64 or 128.  The handle holds no memory of the device. */
+typedef struct gpx_kv_cache gpx_kv_cache;
+int gpx_kv_cache_create(void *k, void *v, void *k_scale, void *v_scale, int pages, int page_tokens, int kv_heads,
+                        int head_dim, gpx_kv_cache **cache);
+int gpx_kv_cache_destroy(gpx_kv_cache *cache);
+
+/* A ragged batch of at most 4096 sequences; the arrays are int32 on the device.  Sequence s has context[s] tokens,
+ * the new ones of this step among them, in the pages table[s][0], table[s][1], ... (table_ld page numbers a row);
+ * its new tokens are rows first[s] .. first[s + 1] - 1 of the step's tensors (none is allowed) and the last ones of
+ * the sequence.  `tokens` rows there are in all, `most_new` of one sequence at most. */
+typedef struct gpx_kv_batch {
+    const void *table, *context, *first;
+    int table_ld, seqs, tokens, most_new;
+} gpx_kv_batch;
+
+/* Appends the step's keys and values to the cache and turns queries and keys by their positions on the way.
+ * q [token][heads][head_dim], k and v [token][kv_heads][head_dim] are "bfloat16" or "float16" with q_ld, k_ld, v_ld
+ * elements from one token to the next (0: packed; multiples of 4, 8-byte aligned); q_out receives the turned queries
+ * in the same type (q and q_out may both be NULL, and may be the same).
+ * Rotation by position p turns pairs (a, b) of the first `rotated` elements of a head (a multiple of 8, 0: none):
+ * a' = a cos - b sin, b' = b cos + a sin with cos[p][j], sin[p][j] of the float tables [positions][rotated / 2]
+ * (16-byte aligned); pair j is elements j and j + rotated / 2, or with `paired` 2 j and 2 j + 1.
+ * The scale of a page and head is the smallest power of two with which its largest finite element is at most 448
+ * (2^-126 at least).  A page that gains larger elements gets a larger scale, and what it holds already is rounded
+ * again to that (exact but for elements that leave the normal range of e4m3); the scale of a page whose first slot
+ * is written starts afresh.  What is not finite is stored as NaN. */
+typedef struct gpx_kv_append_args {
+    const void *q, *k, *v;
+    void *q_out;
+    const void *cos, *sin;
+    long long q_ld, k_ld, v_ld, q_out_ld;
+    int heads, rotated, positions, paired;
+    const char *dtype;
+} gpx_kv_append_args;
+int gpx_kv_append(const gpx_kv_cache *cache, const gpx_kv_batch *batch, const gpx_kv_append_args *args, void *ctx,
+                  const gpx_blp *blp, gpx_stream s);
+
+/* Attention of the new tokens over their sequences' pages: out = softmax(scale q k^T) v for each head, `heads` a
+ * multiple of the cache's kv_heads (consecutive heads share one).  q and out [token][heads][head_dim] are
+ * "bfloat16" or "float16" with q_ld, out_ld elements from one token to the next (0: packed; multiples of 8, 16-byte
+ * aligned); lse, if not NULL, receives the logarithm of each row's normaliser, float [token][heads].
+ * With `causal` token i of n new ones in a context of c sees keys 0 .. c - n + i, otherwise all c (cross attention
+ * over states that were appended once); with `window` > 0 (causal only) only the last `window` of them.  A row
+ * that sees no key is zero, its lse -infinity.  What lies in slots and pages beyond that, NaN codes too, has no
+ * influence.  scale 0 stands for 1 / sqrt(head_dim). */
+typedef struct gpx_kv_attend_args {
+    const void *q;
+    void *out, *lse;
+    long long q_ld, out_ld;
+    int heads, causal, window;
+    float scale;
+    const char *dtype;
+} gpx_kv_attend_args;
+int gpx_kv_attend(const gpx_kv_cache *cache, const gpx_kv_batch *batch, const gpx_kv_attend_args *args, void *ctx,
+                  const gpx_blp *blp, gpx_stream s);
+
+/* Log probabilities from logits [rows][vocab] ("float32", "bfloat16" or "float16", ld elements from row to row, 0:
+ * vocab), each multiplied by inv_temperature (> 0) first.  Any of the outputs may be NULL.
+ *   logprob[row]   of targets[row] (int32; needs targets): 0 for a negative target (no token to score), NaN for one
+ *                  at or past vocab;
+ *   entropy[row]   of the distribution, in nats;
+ *   lse[row]       the logarithm of the normaliser;
+ *   top_ids, top_logprob [row][top]: the `top` (at most 32, and vocab) most likely tokens, equal ones by lowest id.
+ * Logits of -infinity have no probability; a row of nothing else has lse -infinity and NaN elsewhere.  NaN makes a row's figures NaN
+ * and ranks first among the alternatives. */
+typedef struct gpx_token_scores_args {
+    const void *logits, *targets;
+    void *logprob, *entropy, *lse, *top_ids, *top_logprob;
+    long long ld;
+    int rows, vocab, top;
+    float inv_temperature;
+    const char *dtype;
+} gpx_token_scores_args;
+int gpx_token_scores(const gpx_token_scores_args *args, void *ctx, const gpx_blp *blp, gpx_stream s);
+
 /* ---- seeded synthetic data ---------------------------------------------------------- */
 
 /* Counter-based generator: element i of `stream` under `seed` is a pure function of
