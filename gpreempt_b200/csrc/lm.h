@@ -21,7 +21,7 @@ namespace gpx {
 
 // Header, arrival counters (zero between launches: whoever joins the parts of a result puts its counter back), and
 // the parts of results that several CTAs share.
-constexpr int kLmCounters = 8192;
+constexpr int kLmCounters = 65536;
 constexpr size_t kLmPartsOffset = 256 + kLmCounters * sizeof(int);
 constexpr size_t kLmPartsBytes = (size_t)64 << 20;
 constexpr size_t kLmCtxBytes = kLmPartsOffset + kLmPartsBytes;
