@@ -9,8 +9,12 @@
 // operand elements are contiguous bytes, because the order of a contraction's index is free as long as both sides
 // agree on it, and a transposed operand only has to pair the bytes of two keys.  Queries become halves after a power
 // of two that brings their row's largest to 1; the scores' factors (that power, the page's scale, scale, log2 e) are
-// applied to the sums.  Probabilities of fp16 results go through the tensor cores in two halves (22 bits), those of bf16
-// results in one (11 bits against the result's 8).  Statistics and sums are float.
+// applied to the sums.
+//
+// The values' scales join the exponents: what multiplies a code is 2^(s_rj + b_j - M_r), b_j = log2 v_scale, with M the running
+// maximum of s + b, so that the largest factor is 1 and none that counts leaves the range of a half, however far apart
+// the scales of pages are; the normaliser adds it times 2^(-b_j).  Factors of fp16 results go through the tensor cores in
+// two halves (22 bits), those of bf16 results in one (11 bits against the result's 8).  Statistics and sums are float.
 //
 // Four warps take sixteen keys each of a block of 64, with a running maximum and output of their own, and are merged
 // at the end of a unit (a sequence, a head of keys, a block of rows); a fifth keeps the ring of blocks full by TMA,
@@ -19,12 +23,10 @@
 // Work is cut evenly, whatever the sequences' lengths: the blocks of all units lie on one line, and a tile is
 // an equal piece of it.  A unit that spans several tiles leaves their parts in the context, and the
 // CTA that brings the last one joins them in the order of the line.
-#include "lm.h"
+#include "kv_attend.h"
 #include "sm100.cuh"
 
 #include <algorithm>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace gpx {
 
@@ -33,23 +35,6 @@ using namespace sm100;
 constexpr int kAttWarps = 4, kAttConsumers = 32 * kAttWarps, kAttThreads = kAttConsumers + 32;
 constexpr int kAttKeys = 64;
 constexpr unsigned long long kAttWaitNs = 2000000000ull;
-
-struct AttendParams {
-    CUtensorMap map_k, map_v;
-    LmBatch batch;
-    const float *k_scale, *v_scale;
-    int pages, page_shift, kv_heads, heads;
-    const unsigned short *q;
-    unsigned short *out;
-    float *lse;
-    long long q_ld, out_ld;
-    float scale;
-    int causal, window;
-    int max_tiles;
-    int blocks_a_tile;  // of a preemptible launch; 0: as many tiles as CTAs
-    int *error, *counters;
-    float *parts;
-};
 
 template <int D, int NT>
 struct AttCfg {
@@ -66,7 +51,7 @@ struct AttCfg {
 template <int NT>
 struct AttCtl {
     unsigned long long full[8], empty[8];
-    float scales[8][4][2];  // of a stage's sixteen keys of each warp: keys' and values'
+    float scales[8][4][2];  // of a stage's sixteen keys of each warp: keys' scale, log2 of the values'
     float row_factor[8 * NT];
     float ml[kAttWarps][8 * NT][2];
     int tile, last, abort_flag;
@@ -86,11 +71,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-__device__ __forceinline__ uint32_t pack_halves(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_halves(uint32_t w) { return __half22float2(*reinterpret_cast<__half2 *>(&w)); }
 __device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -101,52 +81,6 @@ __device__ __forceinline__ uint2 lds_u2(uint32_t addr) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
-// 0xff in every byte that is e4m3's NaN (all bits but the sign)
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
-
-// A unit's place on the line of blocks, and what it covers.
-struct Unit {
-    int s, head, row0, rows;      // sequence, head of keys, first of its rows and how many
-    int first, n, context;
-    int key0;                     // of its first block (a multiple of 64)
-    int low, high;                // keys that some row sees: [low, high)
-};
-
-template <int ROWS>
-struct Layout {
-    const AttendParams &p;
-    int group;
-    __device__ Layout(const AttendParams &p_) : p(p_), group(p_.heads / p_.kv_heads) {}
-    __device__ int row_blocks(int n) const { return (n * group + ROWS - 1) / ROWS; }
-    // blocks of 64 keys of each unit of a sequence: the most that one of its blocks of rows can see, one at least
-    __device__ int key_blocks(const LmSpan &span) const {
-        int keys = span.context;
-        // (rows of a block span so many tokens; the first key need not start a block)
-        if (p.window) keys = min((long long)keys, (long long)p.window + (ROWS - 1 + group - 1) / group + kAttKeys - 1);
-        return max(1, (keys + kAttKeys - 1) / kAttKeys);
-    }
-    __device__ int line(const LmSpan &span) const {
-        const long long all = (long long)row_blocks(span.n) * p.kv_heads * key_blocks(span);
-        return all > 0x7fffffff ? 0x7fffffff : (int)all;
-    }
-    __device__ Unit unit(int s, int index) const {
-        Unit u;
-        u.s = s;
-        u.first = p.batch.first[s], u.n = p.batch.first[s + 1] - u.first, u.context = p.batch.context[s];
-        const int blocks = row_blocks(u.n);
-        u.head = index / blocks, u.row0 = (index - u.head * blocks) * ROWS;
-        u.rows = min(ROWS, u.n * group - u.row0);
-        u.low = 0, u.high = u.context;
-        if (p.causal) {
-            u.high = max(0, u.context - u.n + (u.row0 + u.rows - 1) / group + 1);
-            if (p.window) u.low = max(0, u.context - u.n + u.row0 / group - p.window + 1);
-        }
-        u.low = min(u.low, u.high);
-        u.key0 = u.low & ~(kAttKeys - 1);
-        return u;
-    }
-};
-
 template <int D, int NT, bool HALF>
 __global__ void __launch_bounds__(kAttThreads)
 kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
@@ -173,7 +107,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     pdl_enter();
     const bool dynamic = blp.preempted != nullptr;
     if (tid == 0) trace_begin(blp);
-    const Layout<ROWS> lay(p);
+    const Layout<ROWS, kAttKeys> lay(p);
     const int group = lay.group, page_tokens = 1 << p.page_shift;
     const int n_line = lm_prefix(prefix, p.batch.seqs, p.error, [&](int s) {
         return lay.line(lm_span(p.batch, s, page_tokens, false, p.error));
@@ -233,13 +167,13 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     const int mine = lane / pieces, sub = lane - mine * pieces;
                     const int key = u.key0 + (block0 + b0 + mine) * kAttKeys + sub * per_page;
                     int row = -1;
-                    float ks = 1.f, vs = 1.f;
+                    float ks = 1.f, vs = 0.f;
                     if (b0 + mine < blocks_live && key < u.high) {
                         const int page = p.batch.table[(size_t)u.s * p.batch.table_ld + (key >> p.page_shift)];
                         if ((unsigned)page < (unsigned)p.pages) {
                             const long long block = (long long)page * p.kv_heads + u.head;
                             row = (int)((block << p.page_shift) + (key & (page_tokens - 1)));
-                            ks = p.k_scale[block], vs = p.v_scale[block];
+                            ks = p.k_scale[block], vs = log2f(fmaxf(p.v_scale[block], 1.17549435e-38f));
                         } else {
                             lm_fail(p.error, LM_BAD_PAGE, u.s);
                         }
@@ -350,12 +284,13 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 const int pos0 = u.context - u.n + u.row0 / group, pos1 = u.context - u.n + (u.row0 + u.rows - 1) / group;
                 const int all_hi = p.causal ? min(u.context, pos0 + 1) : u.context;
                 const int all_lo = p.window ? pos1 + 1 - p.window : 0;
-                float unit_scale = 0.f, most_scale = 0.f;  // what o counts in, and the largest so far
+                // log2 of value scales: of the first block (the normaliser counts in it), the largest, what `times` belongs to
+                float first_b = 0.f, most_b = -INFINITY, times_b = 0.f, times = 1.f;
 
                 for (int b = 0; b < blocks_live; ++b) {
                     wait(&ctl->full[stage], phase);
                     const uint32_t sk = ring + stage * 2 * Cfg::kTile, sv = sk + Cfg::kTile;
-                    const float ks = ctl->scales[stage][wid][0], vs_raw = ctl->scales[stage][wid][1];
+                    const float ks = ctl->scales[stage][wid][0], b_true = ctl->scales[stage][wid][1];
                     const int row16 = wid * 16;
                     const int key0 = u.key0 + (block0 + b) * kAttKeys + row16;
                     // ---- S^T
@@ -396,14 +331,19 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 #pragma unroll
                             for (int c = 0; c < 4; ++c) sc[0][c] += odd[c];
                     }
-                    // ---- scores: factors, masks where a row's border lies in the block
+                    // ---- scores: factors, masks where a row's border lies in the block.  A scale 2^40 below the largest counts
+                    // as that (or its keys would vanish from the normaliser) and the rest goes into the operand.
+                    if (most_b == -INFINITY) first_b = b_true;
+                    most_b = fmaxf(most_b, b_true);
+                    const float b_used = fmaxf(b_true, most_b - 40.f);
+                    if (b_used != times_b || b == 0) times_b = b_used, times = lm_ex2(first_b - b_used);
                     const int block_key = u.key0 + (block0 + b) * kAttKeys;
                     const bool border = block_key + kAttKeys > all_hi || block_key < all_lo;
                     uint32_t seen = ~0u;  // bit 4 nt + c
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) sc[nt][c] *= mult[nt][c & 1] * ks;
+                        for (int c = 0; c < 4; ++c) sc[nt][c] = fmaf(sc[nt][c], mult[nt][c & 1] * ks, b_used);
                     if (border) {
                         const int ka = key0 + key_row(g), kb = ka + 8;
 #pragma unroll
@@ -436,25 +376,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                                 for (int i = 0; i < MT; ++i) o[nt][i][c] *= f, o[nt][i][c + 2] *= f;
                             }
                     }
-                    // ---- the scale of these values (powers of two: o changes its unit exactly; one that is 2^60 below the
-                    // largest so far goes into the probabilities instead, so that o stays finite)
-                    const float vs = fmaxf(vs_raw, 1.17549435e-38f);
-                    float p_factor = 1.f;
-                    if (vs != unit_scale) {
-                        most_scale = fmaxf(most_scale, vs);
-                        const float now = fmaxf(vs, most_scale * 8.673617379884035e-19f);
-                        if (now != unit_scale) {
-                            const float f = unit_scale / now;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                                    for (int c = 0; c < 4; ++c) o[nt][i][c] *= f;
-                            unit_scale = now;
-                        }
-                        p_factor = vs / now;
-                    }
+                    const float p_factor = b_used != b_true ? lm_ex2(b_true - b_used) : 1.f;
                     uint32_t pb[NT][2], pl[kTwo ? NT : 1][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -464,7 +386,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                             const float ref = m[nt][c & 1] == -INFINITY ? 0.f : m[nt][c & 1];
                             e[c] = lm_ex2(sc[nt][c] - ref);
                         }
-                        l[nt][0] += e[0] + e[2], l[nt][1] += e[1] + e[3];
+                        l[nt][0] = fmaf(e[0] + e[2], times, l[nt][0]), l[nt][1] = fmaf(e[1] + e[3], times, l[nt][1]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) e[c] *= p_factor;
                         const uint32_t a = pack_halves(e[0], e[1]), c = pack_halves(e[2], e[3]);
@@ -542,7 +464,12 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     }
                 }
 
-                // ---- the four warps' results as one: warps 2 and 3 into 0 and 1, 1 into 0
+                // ---- the four warps' results as one: warps 2 and 3 into 0 and 1, 1 into 0.  l counts in 2^(m - first_b).
+                const float unit_scale = lm_ex2(first_b);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) m[nt][c] -= first_b;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -611,11 +538,6 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     const int at = u.row0 + r;
                     return p.lse + (long long)(u.first + at / group) * p.heads + u.head * group + at % group;
                 };
-                auto pack_out = [&](float a, float b) {
-                    if (HALF) return pack_halves(a, b);
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-                    return *reinterpret_cast<const uint32_t *>(&h);
-                };
                 const bool whole = blocks == unit_blocks;
                 constexpr int kSlot = ROWS * (D + 2);  // floats: maxima, sums, outputs
                 if (wid == 0) {
@@ -633,7 +555,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 #pragma unroll
                                 for (int i = 0; i < MT; ++i) {
                                     const float a = o[nt][i][c], b = o[nt][i][c + 2];
-                                    w[i] = inv == 0.f ? 0u : pack_out(a * inv, b * inv);
+                                    w[i] = inv == 0.f ? 0u : pack_out<HALF>(a * inv, b * inv);
                                 }
                                 uint4 *to = reinterpret_cast<uint4 *>(out_row(r) + g * (D / 8));
 #pragma unroll
@@ -695,7 +617,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                         finish_row(r, mm, all, inv, log_sum);
                         uint32_t w[D / 64];
 #pragma unroll
-                        for (int j = 0; j < D / 64; ++j) w[j] = inv == 0.f ? 0u : pack_out(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+                        for (int j = 0; j < D / 64; ++j) w[j] = inv == 0.f ? 0u : pack_out<HALF>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
                         uint32_t *to = reinterpret_cast<uint32_t *>(out_row(r)) + lane * (D / 64);
                         if (D == 128) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[D / 64 - 1]);
                         else to[0] = w[0];
@@ -728,9 +650,12 @@ static auto attend_instance(int dim, int rows, bool half, F &&f) {
     return half ? by_rows(D128(), std::true_type()) : by_rows(D128(), std::false_type());
 }
 
+// Rows of a head of keys (its group's heads times the tokens) from which on the other kernel takes over.
+constexpr int kManyRows = 32;
+
 constexpr int kBlocksATile = 16;  // of a preemptible launch: 1024 keys, 256 KiB of a head of 128
 
-static cudaError_t attend_launch(AttendParams &p, int dim, bool half, const DeviceInfo &d, const BlpArgs &blp, cudaStream_t s) {
+cudaError_t kv_attend_few_launch(AttendParams &p, int dim, bool half, const DeviceInfo &d, const BlpArgs &blp, cudaStream_t s) {
     const int rows = (int)std::min<long long>((long long)p.batch.most_new * (p.heads / p.kv_heads), 1 << 20);
     return attend_instance(dim, rows, half, [&](auto kernel, size_t smem, int tile_rows) {
         smem += (p.batch.seqs + 1) * sizeof(int);
@@ -775,13 +700,14 @@ extern "C" int gpx_kv_attend(const gpx_kv_cache *cache, const gpx_kv_batch *batc
     GPX_REQUIRE(d.device >= 0, GPX_FAIL, "gpx_init was not called");
     if (p.batch.most_new == 0) return GPX_SUCC;
     p.map_k = cache->map_k, p.map_v = cache->map_v;
-    p.k_scale = cache->k_scale, p.v_scale = cache->v_scale;
+    p.v_codes = cache->v, p.k_scale = cache->k_scale, p.v_scale = cache->v_scale;
     p.pages = cache->pages, p.page_shift = __builtin_ctz((unsigned)cache->page_tokens), p.kv_heads = cache->kv_heads, p.heads = a.heads;
     p.q = (const unsigned short *)a.q, p.out = (unsigned short *)a.out, p.lse = (float *)a.lse;
     p.scale = a.scale != 0.f ? a.scale : 1.0f / sqrtf((float)cache->dim);
     p.causal = a.causal != 0, p.window = a.window;
     const LmCtx c = lm_ctx(ctx);
     p.error = c.error, p.counters = c.counters, p.parts = c.parts;
-    GPX_CUDA(attend_launch(p, cache->dim, elem == LM_F16, d, b, as_stream(stream)));
+    const bool many = (long long)p.batch.most_new * (a.heads / cache->kv_heads) > kManyRows;
+    GPX_CUDA((many ? kv_attend_many_launch : kv_attend_few_launch)(p, cache->dim, elem == LM_F16, d, b, as_stream(stream)));
     return GPX_SUCC;
 }
