@@ -706,7 +706,7 @@ extern "C" int gpx_kv_attend(const gpx_kv_cache *cache, const gpx_kv_batch *batc
     p.scale = a.scale != 0.f ? a.scale : 1.0f / sqrtf((float)cache->dim);
     p.causal = a.causal != 0, p.window = a.window;
     const LmCtx c = lm_ctx(ctx);
-    p.error = c.error, p.counters = c.counters, p.parts = c.parts;
+    p.error = c.error, p.counters = c.counters, p.prefix = c.prefix, p.parts = c.parts;
     const bool many = (long long)p.batch.most_new * (a.heads / cache->kv_heads) > kManyRows;
     GPX_CUDA((many ? kv_attend_many_launch : kv_attend_few_launch)(p, cache->dim, elem == LM_F16, d, b, as_stream(stream)));
     return GPX_SUCC;

@@ -22,7 +22,7 @@ struct AttendParams {
     int causal, window;
     int max_tiles;
     int blocks_a_tile;  // of a preemptible launch; 0: as many tiles as CTAs
-    int *error, *counters;
+    int *error, *counters, *prefix;
     float *parts;
 };
 

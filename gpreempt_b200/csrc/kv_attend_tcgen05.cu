@@ -36,12 +36,14 @@ constexpr int kManyThreads = 512;  // two warpgroups of rows, one that converts,
 // registers of a thread of the first two and of the others: together what the CTA was launched with, 128 a thread
 constexpr int kManyRegs = 168, kFewRegs = 88;
 constexpr int kTileRows = 256, kTileKeys = 128;
-constexpr int kRawStages = 3, kValueBuffers = 2;  // (a stage of the ring holds a block's keys or its values)
+constexpr int kRawStages = 2, kKeyBuffers = 2, kValueBuffers = 2;  // (a stage of the ring holds a block's keys or its values)
 constexpr unsigned long long kManyWaitNs = 2000000000ull;
-// How far, in powers of two, a row's maximum may be above the reference of its exponents before they are taken anew and the sums
-// rescaled.  With 0 that happens in most blocks (a new maximum of one row in 32), and a block is gone through twice: once for
-// its maximum, once for the exponentials.
-constexpr float kLag = 8.f;
+// A row's exponents refer to its maximum in the first block it sees until their factors sum to more than this in a block, which a
+// half holds; then the maximum is taken anew and the sums are rescaled.  (Asking for the maximum of every block goes
+// through its scores twice, and a new one among 32 rows, which are rescaled together, comes in most blocks.)
+constexpr float kMostFactors = 32768.f;
+// Blocks of the longest unit up to which units are not cut.
+constexpr int kShortUnit = 8;
 constexpr int kNotes = 1024;  // the last counters of the context: {tile + 1, blocks done, whether sums were left} of a CTA's unfinished tile
 
 template <int D>
@@ -49,14 +51,14 @@ struct ManyCfg {
     static constexpr uint32_t kQ = 128 * D * 2;            // of a warpgroup
     static constexpr uint32_t kHalves = kTileKeys * D * 2;  // keys or values of a block, as halves
     static constexpr uint32_t kCodes = kTileKeys * D;
-    static constexpr uint32_t kKeysAt = 2 * kQ, kValuesAt = kKeysAt + kHalves, kRawAt = kValuesAt + kValueBuffers * kHalves;
+    static constexpr uint32_t kKeysAt = 2 * kQ, kValuesAt = kKeysAt + kKeyBuffers * kHalves, kRawAt = kValuesAt + kValueBuffers * kHalves;
     static constexpr uint32_t kCtlAt = kRawAt + kRawStages * kCodes;
     static constexpr int kSlot = 2 * kTileRows + kTileRows * D;  // floats: maxima, sums, outputs [D / 4][row][4]
 };
 
 struct ManyCtl {
     unsigned long long raw_full[kRawStages], raw_empty[kRawStages];
-    unsigned long long keys_full, keys_empty;
+    unsigned long long keys_full[kKeyBuffers], keys_empty[kKeyBuffers];
     unsigned long long values_full[kValueBuffers], values_empty[kValueBuffers];
     unsigned long long s_full[2], p_full[2];
     alignas(16) float scales[4][8][4];  // of a block's sixteen keys each: keys' and values' scale, b = log2 of the values' over the largest, 2^-b
@@ -65,7 +67,7 @@ struct ManyCtl {
     int tile, done, spilled;  // the tile, the blocks of it that an earlier launch has done, and whether the last unit's sums were left
     int end;                  // the block of the unit at which the piece ends
     int stopped;              // because of the word
-    int saw_nan, last, abort_flag;
+    int saw_nan, last, longest, abort_flag;
 };
 
 // The largest of three (one instruction on this architecture).
@@ -95,14 +97,14 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     ManyCtl *ctl = reinterpret_cast<ManyCtl *>(smem + Cfg::kCtlAt);
-    int *prefix = reinterpret_cast<int *>(ctl + 1);  // [seqs + 1]
+    int *const prefix = p.prefix;  // [seqs + 1], the same from every CTA (shared memory is full)
     volatile int *abort_flag = &ctl->abort_flag;
     const uint32_t base = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, wid = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const bool elected = elect_one();
     if (tid == 0) {
         for (int i = 0; i < kRawStages; ++i) mbar_init(smem_u32(&ctl->raw_full[i]), 1), mbar_init(smem_u32(&ctl->raw_empty[i]), 4);
-        mbar_init(smem_u32(&ctl->keys_full), 4), mbar_init(smem_u32(&ctl->keys_empty), 1);
+        for (int i = 0; i < kKeyBuffers; ++i) mbar_init(smem_u32(&ctl->keys_full[i]), 4), mbar_init(smem_u32(&ctl->keys_empty[i]), 1);
         for (int i = 0; i < kValueBuffers; ++i) mbar_init(smem_u32(&ctl->values_full[i]), 4), mbar_init(smem_u32(&ctl->values_empty[i]), 1);
         for (int w = 0; w < 2; ++w) {
             mbar_init(smem_u32(&ctl->s_full[w]), 1), mbar_init(smem_u32(&ctl->p_full[w]), 4);
@@ -131,28 +133,47 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 
     // ---- the line of blocks
     auto blocks_of = [&](const Unit &u) { return max(1, (u.high - u.key0 + kTileKeys - 1) / kTileKeys); };
-    // (sequences of many blocks of rows are counted by a warp, the others by a thread)
+    // (Sequences of many blocks of rows are counted by a warp, the others by a thread.  Counts and sums are made where
+    // the queries will lie; the sums then go to the context, and no CTA ever writes anything else there.)
+    int *const count = reinterpret_cast<int *>(smem);
+    if (tid == 0) ctl->longest = 0;
+    __syncthreads();
     for (int s = tid; s < p.batch.seqs; s += kManyThreads) {
         const LmSpan span = lm_span(p.batch, s, page_tokens, false, p.error);
         const int rows = lay.row_blocks(span.n);
         long long all = rows > 8 ? -1 : 0;
-        for (int i = 0; all >= 0 && i < rows; ++i) all += blocks_of(lay.unit(s, i));
-        prefix[s] = (int)min(all < 0 ? all : all * p.kv_heads, 0x7fffffffll);
+        for (int i = 0; all >= 0 && i < rows; ++i) {
+            const int blocks = blocks_of(lay.unit(s, i));
+            if (blocks > kShortUnit) ctl->longest = blocks;
+            all += blocks;
+        }
+        count[s] = (int)min(all < 0 ? all : all * p.kv_heads, 0x7fffffffll);
     }
     __syncthreads();
     for (int s = wid; s < p.batch.seqs; s += kManyThreads / 32) {
-        if (prefix[s] >= 0) continue;
+        if (count[s] >= 0) continue;
         const int rows = lay.row_blocks(p.batch.first[s + 1] - p.batch.first[s]);
         long long all = 0;
-        for (int i = lane; i < rows; i += 32) all += blocks_of(lay.unit(s, i));
+        for (int i = lane; i < rows; i += 32) {
+            const int blocks = blocks_of(lay.unit(s, i));
+            if (blocks > kShortUnit) ctl->longest = blocks;
+            all += blocks;
+        }
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-        if (lane == 0) prefix[s] = (int)min(all * p.kv_heads, 0x7fffffffll);
+        if (lane == 0) count[s] = (int)min(all * p.kv_heads, 0x7fffffffll);
     }
     __syncthreads();
-    const int n_line = lm_prefix(prefix, p.batch.seqs, p.error, [&](int s) { return prefix[s]; });
-    const int tiles = min(n_line, (int)gridDim.x);
+    // Units of a few blocks each are tiles as they are: joining their parts would take longer than their blocks.
+    const bool by_unit = ctl->longest == 0;
+    const int n_line = lm_prefix(count, p.batch.seqs, p.error, [&](int s) {
+        return by_unit && count[s] ? lay.row_blocks(p.batch.first[s + 1] - p.batch.first[s]) * p.kv_heads : count[s];
+    });
+    for (int s = tid; s <= p.batch.seqs; s += kManyThreads) prefix[s] = n_line ? count[s] : 0;
+    __syncthreads();
+    const int tiles = by_unit ? n_line : min(n_line, (int)gridDim.x);
     blp.total_tiles = tiles;
+    auto on_line = [&](const Unit &u) { return by_unit ? 1 : blocks_of(u); };  // what a unit takes of the line
     auto tile_begin = [&](int t) { return (int)((long long)t * n_line / tiles); };
     auto tile_of = [&](int b) { return (int)((((long long)b + 1) * tiles - 1) / n_line); };
     int *const note = p.counters + kLmCounters - kNotes + 4 * blockIdx.x;
@@ -192,14 +213,15 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             x.line0 = tile_begin(x.tile);
             const int line1 = tile_begin(x.tile + 1);
             // the first unit: its sequence, head and block of rows
-            int at = x.line0 + ctl->done;
+            // (where a unit is a tile, its place on the line is not that of its blocks: what is done of it is added below)
+            int at = x.line0 + (by_unit ? 0 : ctl->done);
             int s = lm_find(prefix, p.batch.seqs, at);
             int rb_count = lay.row_blocks(p.batch.first[s + 1] - p.batch.first[s]), rb = 0;
             const int a_head = (prefix[s + 1] - prefix[s]) / p.kv_heads;
             int head = (at - prefix[s]) / a_head;
             x.unit0 = prefix[s] + head * a_head;
             for (;; rb += 32) {
-                int upto = rb + lane < rb_count ? blocks_of(lay.unit(s, rb + lane)) : 0;
+                int upto = rb + lane < rb_count ? on_line(lay.unit(s, rb + lane)) : 0;
                 const int own = upto;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -219,7 +241,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             for (;;) {
                 x.u = lay.unit(s, head * rb_count + rb);
                 x.unit_blocks = blocks_of(x.u);
-                x.b0 = max(x.line0 - x.unit0, 0), x.b1 = min(line1 - x.unit0, x.unit_blocks), x.done = at - x.unit0;
+                if (by_unit) x.b0 = 0, x.b1 = x.unit_blocks, x.done = ctl->done;
+                else x.b0 = max(x.line0 - x.unit0, 0), x.b1 = min(line1 - x.unit0, x.unit_blocks), x.done = at - x.unit0;
                 x.blocks = min(x.b1, max(0, (x.u.high - x.u.key0 + kTileKeys - 1) / kTileKeys));
                 x.whole = x.b0 == 0 && x.b1 == x.unit_blocks, x.ran = ran;
                 x.two = x.u.rows > 128;
@@ -232,7 +255,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 tc_fence_after_sync();
                 if (ctl->stopped) {
                     if (tid == 0) {
-                        note[0] = x.tile + 1, note[1] = x.unit0 + ctl->end - x.line0, note[2] = ctl->end > x.b0;
+                        note[0] = x.tile + 1, note[1] = by_unit ? ctl->end : x.unit0 + ctl->end - x.line0, note[2] = ctl->end > x.b0;
                         atomicCAS(blp.stop_index, -1, blp.kernel_id);
                     }
                     return;
@@ -251,7 +274,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 }
                 if (*abort_flag) return;
                 // ---- the next unit of the tile
-                x.unit0 += x.unit_blocks;
+                x.unit0 += on_line(x.u);
                 ran = true;
                 if (x.unit0 >= line1) break;
                 at = x.unit0, x.goes_on = false;
@@ -354,7 +377,9 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             if (w == 0 || x.two) wait(&ctl->p_full[w], n_p[w]++ & 1);
         for (int j = x.done;; ++j) {
             // scores of block j, the products with the values of block j - 1 before them
-            wait(&ctl->keys_full, n_keys++ & 1);
+            const int keys = n_keys % kKeyBuffers;
+            wait(&ctl->keys_full[keys], n_keys / kKeyBuffers & 1);
+            ++n_keys;
             tc_fence_after_sync();
             const bool ends = ended(j), has_values = j > x.done;
             const int buffer = n_values % kValueBuffers;
@@ -378,7 +403,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 }
                 if (!ends) {
                     if (elected && !*abort_flag) {
-                        const uint64_t dq = make_smem_desc_sw128(base + w * Cfg::kQ), dk = make_smem_desc_sw128(base + Cfg::kKeysAt);
+                        const uint64_t dq = make_smem_desc_sw128(base + w * Cfg::kQ), dk = make_smem_desc_sw128(base + Cfg::kKeysAt + keys * Cfg::kHalves);
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
                             const uint32_t step = (k & 3) * 2 + (k >> 2) * (kHalfTile >> 4);
@@ -393,7 +418,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 commit(&ctl->values_empty[buffer]);
                 ++n_values;
             }
-            commit(&ctl->keys_empty);
+            commit(&ctl->keys_empty[keys]);
             if (ends) break;
         }
     };
@@ -455,13 +480,15 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 const float used = fmaxf(fmaxf(ctl->scales[j & 3][r][1], 1.17549435e-38f) / most, 9.094947e-13f);
                 ctl->scales[j & 3][r][2] = log2f(used), ctl->scales[j & 3][r][3] = 1.f / used;
             }
-            wait(&ctl->keys_empty, (n_keys++ & 1) ^ 1);
+            const int keys = n_keys % kKeyBuffers;
+            wait(&ctl->keys_empty[keys], (n_keys / kKeyBuffers & 1) ^ 1);
+            ++n_keys;
             if (!ends) {
-                rows(smem + Cfg::kRawAt + st * Cfg::kCodes, smem + Cfg::kKeysAt);
+                rows(smem + Cfg::kRawAt + st * Cfg::kCodes, smem + Cfg::kKeysAt + keys * Cfg::kHalves);
                 fence_proxy_async();
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&ctl->raw_empty[st])), mbar_arrive(smem_u32(&ctl->keys_full));
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->raw_empty[st])), mbar_arrive(smem_u32(&ctl->keys_full[keys]));
             ++n_raw;
             if (ends) break;
             st = n_raw % kRawStages;
@@ -578,80 +605,85 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             const bool masks = x.border(j);
             const int high = hi - x.key(j), low = lo - x.key(j);
             auto hide = [&](int c, uint32_t(&v)[32]) {
-                if (masks) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * c + i >= high || 32 * c + i < low) v[i] = 0xff800000u;
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (32 * c + i >= high || 32 * c + i < low) v[i] = 0xff800000u;
             };
-            auto largest_of = [&](const uint32_t *e) {  // of sixteen
-                float a = max3(__uint_as_float(e[0]), __uint_as_float(e[1]), __uint_as_float(e[2]));
-                float b = max3(__uint_as_float(e[3]), __uint_as_float(e[4]), __uint_as_float(e[5]));
-#pragma unroll
-                for (int i = 6; i < 14; i += 4) {
-                    a = max3(a, __uint_as_float(e[i]), __uint_as_float(e[i + 1]));
-                    b = max3(b, __uint_as_float(e[i + 2]), __uint_as_float(e[i + 3]));
-                }
-                return max3(fmaxf(a, b), __uint_as_float(e[14]), __uint_as_float(e[15]));
-            };
-            if (j == x.b0) {
-                // the first block's maximum is the first reference
+            // the largest exponent of the row in this block
+            auto largest = [&]() {
+                float most = -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[32];
                     tmem_ld_32x32(t_s + 32 * c, v);
                     tmem_ld_wait();
-                    hide(c, v);
+                    if (masks) hide(c, v);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const float4 g = of[2 * c + q];
-                        m = fmaxf(m, fmaf(largest_of(v + 16 * q), g.x * mult, g.z));
+                        float e = __uint_as_float(v[16 * q]);
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) e = fmaxf(e, __uint_as_float(v[16 * q + i]));
+                        most = fmaxf(most, fmaf(e, g.x * mult, g.z));
                     }
                 }
-            }
+                return most;
+            };
             uint32_t h[64];
-            float sum;
-            for (;;) {
+            float sum, plain;  // of the factors as the normaliser and as the operand has them
+            auto exponentials = [&](auto masked) {
                 const float ref = m == -INFINITY ? 0.f : m;
-                float most = -INFINITY;
-                sum = 0.f;
+                sum = plain = 0.f;
                 uint32_t both[2][32];
                 tmem_ld_32x32(t_s, both[0]);
+                float4 next[2] = {of[0], of[1]};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t(&v)[32] = both[c & 1];
+                    const float4 g[2] = {next[0], next[1]};
                     tmem_ld_wait();
-                    if (c < 3) tmem_ld_32x32(t_s + 32 * (c + 1), both[(c + 1) & 1]);  // (on its way under this one's exponentials)
-                    hide(c, v);
+                    if (c < 3) {
+                        // (on its way under this one's exponentials)
+                        tmem_ld_32x32(t_s + 32 * (c + 1), both[(c + 1) & 1]);
+                        next[0] = of[2 * c + 2], next[1] = of[2 * c + 3];
+                    }
+                    if (decltype(masked)::value) hide(c, v);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        const float4 g = of[2 * c + q];
-                        most = fmaxf(most, fmaf(largest_of(v + 16 * q), g.x * mult, g.z));
-                        const float2 by = make_float2(g.x * mult, g.x * mult), plus = make_float2(g.z - ref, g.z - ref);
-                        float2 part = make_float2(0.f, 0.f);
+                        const float2 by = make_float2(g[q].x * mult, g[q].x * mult), plus = make_float2(g[q].z - ref, g[q].z - ref);
+                        float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                         for (int i = 8 * q; i < 8 * q + 8; ++i) {
                             const float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, plus);
                             const float2 e = make_float2(lm_ex2(y.x), lm_ex2(y.y));
-                            part = add2(part, e);
+                            part[i & 1] = add2(part[i & 1], e);
                             h[16 * c + i] = pack_halves(e.x, e.y);
                         }
-                        sum = fmaf(part.x + part.y, g.w, sum);
+                        const float all = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                        plain += all, sum = fmaf(all, g[q].w, sum);
                     }
                 }
-                if (!__any_sync(0xffffffffu, most > m + kLag)) break;
+            };
+            // The maximum of the first block that a row sees is its first reference.  Later ones are not asked for theirs: where
+            // the factors of a row sum to less than 2^15 none has left the range of a half.
+            if (__any_sync(0xffffffffu, m == -INFINITY)) {
+                const float most = largest();
+                if (m == -INFINITY) m = most;
+            }
+            for (bool again = masks;; again = true) {
+                if (again) exponentials(std::true_type());
+                else exponentials(std::false_type());
+                if (!__any_sync(0xffffffffu, plain > kMostFactors)) break;
                 // (the scores' arrival means that the products before them are complete)
-                const float now = fmaxf(m, most), f = now == -INFINITY ? 1.f : lm_ex2(m - now);
-                if (j > x.b0) {
+                const float now = fmaxf(m, largest()), f = now == -INFINITY ? 1.f : lm_ex2(m - now);
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tmem_ld_32x32(t_o + c, o);
-                        tmem_ld_wait();
+                for (int c = 0; j > x.b0 && c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32x32(t_o + c, o);
+                    tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st_32x32(t_o + c, o);
-                    }
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st_32x32(t_o + c, o);
                 }
                 l *= f;
                 m = now;
@@ -799,7 +831,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 
 cudaError_t kv_attend_many_launch(AttendParams &p, int dim, bool half, const DeviceInfo &d, const BlpArgs &blp, cudaStream_t s) {
     auto go = [&](auto kernel, uint32_t fixed, int slot) {
-        const size_t smem = 1024 + fixed + sizeof(ManyCtl) + (p.batch.seqs + 1) * sizeof(int);
+        const size_t smem = 1024 + fixed + sizeof(ManyCtl);
         int per_sm;
         const cudaError_t e = lm_resident((const void *)kernel, kManyThreads, smem, d.device, &per_sm);
         if (e != cudaSuccess) return e;

@@ -97,7 +97,7 @@ int gpx_lm_ctx_bytes(size_t *bytes) {
 
 int gpx_lm_ctx_reset(void *ctx, gpx_event *ready) {
     GPX_REQUIRE(ctx, GPX_FAIL, "ctx is NULL");
-    GPX_CUDA(cudaMemsetAsync(ctx, 0, kLmPartsOffset, nullptr));
+    GPX_CUDA(cudaMemsetAsync(ctx, 0, kLmResetBytes, nullptr));
     return record_ready(ready);
 }
 

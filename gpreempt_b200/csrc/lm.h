@@ -20,9 +20,11 @@ namespace gpx {
 // ---- scratch context ------------------------------------------------------------------------------
 
 // Header, arrival counters (zero between launches: whoever joins the parts of a result puts its counter back), and
-// the parts of results that several CTAs share.
+// what CTAs have in common: sums over the sequences of a batch, parts of results.
 constexpr int kLmCounters = 65536;
-constexpr size_t kLmPartsOffset = 256 + kLmCounters * sizeof(int);
+constexpr int kLmMaxSeqs = 4096;
+constexpr size_t kLmResetBytes = 256 + kLmCounters * sizeof(int);
+constexpr size_t kLmPartsOffset = kLmResetBytes + (kLmMaxSeqs + 64) * sizeof(int);
 constexpr size_t kLmPartsBytes = (size_t)64 << 20;
 constexpr size_t kLmCtxBytes = kLmPartsOffset + kLmPartsBytes;
 
@@ -37,17 +39,16 @@ enum LmError {
 struct LmCtx {
     int *error;  // {code, sequence or CTA}
     int *counters;
+    int *prefix;  // [kLmMaxSeqs + 1]
     float *parts;
 };
 
 inline LmCtx lm_ctx(void *ctx) {
     unsigned char *p = static_cast<unsigned char *>(ctx);
-    return {reinterpret_cast<int *>(p), reinterpret_cast<int *>(p + 256), reinterpret_cast<float *>(p + kLmPartsOffset)};
+    return {reinterpret_cast<int *>(p), reinterpret_cast<int *>(p + 256), reinterpret_cast<int *>(p + kLmResetBytes), reinterpret_cast<float *>(p + kLmPartsOffset)};
 }
 
 // ---- batch ----------------------------------------------------------------------------------------
-
-constexpr int kLmMaxSeqs = 4096;
 
 struct LmBatch {
     const int *table;    // [seqs][table_ld] page numbers
