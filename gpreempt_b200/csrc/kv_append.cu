@@ -47,6 +47,9 @@ __device__ __forceinline__ unsigned pack16(float a, float b) {
     return *reinterpret_cast<unsigned *>(&h);
 }
 
+// How rows are turned: all of them in the one order or the other, or as the arguments say.
+enum TurnMode { TURN_HALVES, TURN_PAIRS, TURN_ANY };
+
 // Where lane i of a row keeps its elements: four from a, four from b, and the first of their angles.
 struct Place {
     int a, b;
@@ -69,11 +72,6 @@ __device__ __forceinline__ void decode8(const Raw8 &r, float (&x)[8]) {
     const float2 a0 = unpack16<HALF>(r.a.x), a1 = unpack16<HALF>(r.a.y), b0 = unpack16<HALF>(r.b.x), b1 = unpack16<HALF>(r.b.y);
     x[0] = a0.x, x[1] = a0.y, x[2] = a1.x, x[3] = a1.y, x[4] = b0.x, x[5] = b0.y, x[6] = b1.x, x[7] = b1.y;
 }
-__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s) {
-    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-    b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
-    a = x;
-}
 struct Angles {
     float4 c, s;
 };
@@ -82,8 +80,16 @@ __device__ __forceinline__ Angles angles_of(const AppendParams &p, int pos, int 
     const size_t at = (size_t)pos * (p.rotated / 2) + 4 * i;
     return {__ldg(reinterpret_cast<const float4 *>(p.cos + at)), __ldg(reinterpret_cast<const float4 *>(p.sin + at))};
 }
-__device__ __forceinline__ void turn8(float (&x)[8], const Angles &t, bool paired) {
-    if (paired) {
+// (the products are rounded on their own; as pairs of packed instructions the compiler fuses them with the sums)
+__device__ __forceinline__ void turn_pair(float &a, float &b, float c, float s) {
+    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+    b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+    a = x;
+}
+template <int MODE>
+__device__ __forceinline__ void turn8(float (&x)[8], const Angles &t, const Place &at, bool paired) {
+    if (MODE == TURN_ANY && !at.turned) return;
+    if (MODE == TURN_PAIRS || (MODE == TURN_ANY && paired)) {
         turn_pair(x[0], x[1], t.c.x, t.s.x), turn_pair(x[2], x[3], t.c.y, t.s.y);
         turn_pair(x[4], x[5], t.c.z, t.s.z), turn_pair(x[6], x[7], t.c.w, t.s.w);
     } else {
@@ -92,13 +98,20 @@ __device__ __forceinline__ void turn8(float (&x)[8], const Angles &t, bool paire
     }
 }
 
-// The bits of the largest finite magnitude (as unsigned they are ordered as the numbers are).
-__device__ __forceinline__ unsigned amax8(const float (&x)[8]) {
-    unsigned m = 0;
+// The bits of the largest magnitude (as unsigned they are ordered as the numbers are), of which NaN is none; where it
+// is infinite, that of the finite ones, and `wild` is set.
+__device__ __forceinline__ unsigned amax8(const float (&x)[8], bool &wild) {
+    float a = fmaxf(fabsf(x[0]), fabsf(x[1])), b = fmaxf(fabsf(x[2]), fabsf(x[3]));
+    a = fmaxf(a, fmaxf(fabsf(x[4]), fabsf(x[5]))), b = fmaxf(b, fmaxf(fabsf(x[6]), fabsf(x[7])));
+    unsigned m = __float_as_uint(fmaxf(a, b));
+    if (m >= 0x7f800000u) {
+        wild = true;
+        m = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const unsigned u = __float_as_uint(x[j]) & 0x7fffffffu;
-        if (u < 0x7f800000u) m = max(m, u);
+        for (int j = 0; j < 8; ++j) {
+            const unsigned u = __float_as_uint(x[j]) & 0x7fffffffu;
+            if (u < 0x7f800000u) m = max(m, u);
+        }
     }
     return m;
 }
@@ -107,18 +120,24 @@ __device__ __forceinline__ float scale_for(unsigned amax_bits) {
     const int e = (int)((amax_bits + 0x1fffffu) >> 23) - 8;
     return __uint_as_float((unsigned)max(e, 1) << 23);
 }
-__device__ __forceinline__ unsigned codes4(const float *x, float inv) {
+// (the conversion turns NaN into NaN, but an infinity into the largest code: it is made NaN before)
+__device__ __forceinline__ unsigned codes4(const float *x, float inv, bool wild) {
     float y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const bool finite = (__float_as_uint(x[j]) & 0x7fffffffu) < 0x7f800000u;
-        y[j] = finite ? x[j] * inv : __uint_as_float(0x7fffffffu);
+        y[j] = x[j] * inv;
+        if (wild && (__float_as_uint(x[j]) & 0x7fffffffu) >= 0x7f800000u) y[j] = __uint_as_float(0x7fffffffu);
     }
     return e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16;
 }
-__device__ __forceinline__ void store8(unsigned char *row, const Place &at, const float (&x)[8], float inv) {
-    *reinterpret_cast<unsigned *>(row + at.a) = codes4(x, inv);
-    *reinterpret_cast<unsigned *>(row + at.b) = codes4(x + 4, inv);
+__device__ __forceinline__ void store8(unsigned char *row, const Place &at, const float (&x)[8], float inv, bool wild) {
+    const unsigned a = codes4(x, inv, wild), b = codes4(x + 4, inv, wild);
+    if (at.b == at.a + 4) {
+        *reinterpret_cast<uint2 *>(row + at.a) = make_uint2(a, b);
+    } else {
+        *reinterpret_cast<unsigned *>(row + at.a) = a;
+        *reinterpret_cast<unsigned *>(row + at.b) = b;
+    }
 }
 // Codes of a smaller scale under a larger one (ratio: smaller / larger, a power of two).
 __device__ __forceinline__ unsigned again4(unsigned w, float ratio) {
@@ -184,7 +203,7 @@ kv_append_one_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
             const int h = role - 2 * p.kv_heads;
             const Angles t = angles_of(p, pos, i, at.turned);
             decode8<HALF>(fetch8(p.q + span.first * p.q_ld + h * D, at), x);
-            if (at.turned) turn8(x, t, p.paired);
+            turn8<TURN_ANY>(x, t, at, p.paired);
             unsigned short *out = p.q_out + span.first * p.q_out_ld + h * D;
             *reinterpret_cast<uint2 *>(out + at.a) = make_uint2(pack16<HALF>(x[0], x[1]), pack16<HALF>(x[2], x[3]));
             *reinterpret_cast<uint2 *>(out + at.b) = make_uint2(pack16<HALF>(x[4], x[5]), pack16<HALF>(x[6], x[7]));
@@ -199,13 +218,14 @@ kv_append_one_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
         float *scale_at = (is_v ? p.v_scale : p.k_scale) + (size_t)page * p.kv_heads + h;
         const float old = slot ? *scale_at : 0.f;
         decode8<HALF>(raw, x);
-        if (at.turned) turn8(x, t, p.paired);
-        unsigned m = amax8(x);
+        turn8<TURN_ANY>(x, t, at, p.paired);
+        bool wild = false;
+        unsigned m = amax8(x, wild);
 #pragma unroll
         for (int d = kLanes / 2; d >= 1; d >>= 1) m = max(m, __shfl_xor_sync(mask, m, d));
         const float want = scale_for(m), scale = fmaxf(old, want);
         unsigned char *block = (is_v ? p.v_codes : p.k_codes) + ((size_t)page * p.kv_heads + h) * page_tokens * D;
-        store8(block + slot * D, at, x, 1.0f / scale);
+        store8(block + slot * D, at, x, 1.0f / scale, wild);
         if (scale > old) {
             __syncwarp(mask);  // every lane has read the old scale
             if (i == 0) *scale_at = scale;
@@ -218,14 +238,21 @@ kv_append_one_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
 }
 
 // Any number of new tokens: a tile is what a sequence adds to one page of one head of keys and values, and the
-// queries of that head's group.  Keys and values of the tile stay in registers between the reduction of their
-// amax and their rounding, R rows a lane group of either.
+// queries of that head's group.  Keys and values of the tile wait in shared memory between the reduction of their
+// amax and their rounding.  The queries ride along because they turn by the same angles, which are twice their bytes to read
+// (as tiles of their own, in the order of memory, the whole took 147 us against 126 at the time).
+// What bounds it is latency: loads of a row, a barrier, stores, with 24 warps an SM, and 48 million instructions, half of what
+// the time holds.  Eight prompts of 21 700 tokens in all, 32 heads of 128 on 8: 100 us (533 MB, 5.3 TB/s); with 16 warps 117, with
+// 32 (64 registers) 116, with the rotation's order looked up for each row 119.
 constexpr int kAppendThreads = 256;
-template <int D, int R, bool HALF>
-__global__ void __launch_bounds__(kAppendThreads)
+template <int D, bool HALF, int MODE>
+__global__ void __launch_bounds__(kAppendThreads, 3)
 kv_append_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
-    constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes;
-    extern __shared__ int s_prefix[];  // [seqs + 1]
+    constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes, kHeads = 4;
+    // keys of the tile, turned, and values as they came, each thread's for itself; sums over the sequences [seqs + 1]
+    extern __shared__ float4 keys[];
+    uint4 *const values = reinterpret_cast<uint4 *>(keys + (D / 4 << p.page_shift));
+    int *const s_prefix = reinterpret_cast<int *>(values + (kLanes << p.page_shift));
     __shared__ int s_tile;
     __shared__ unsigned s_amax[2];
     pdl_enter();
@@ -261,45 +288,70 @@ kv_append_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
         const int token0 = span.first + pos0 - (span.context - span.n);
         const int page = page_of(p, s, index);  // (the same for the whole CTA)
         const Place at_k = place_of(p, i, true), at_v = place_of(p, i, false);
+        // the queries of the group for a token
+        auto queries = [&](int row, const Angles &t) {
+            const unsigned short *from_a = p.q + (token0 + row) * p.q_ld + h * group * D + at_k.a, *from_b = from_a + (at_k.b - at_k.a);
+            unsigned short *to_a = p.q_out + (token0 + row) * p.q_out_ld + h * group * D + at_k.a, *to_b = to_a + (at_k.b - at_k.a);
+            auto some = [&](auto heads) {
+                constexpr int N = decltype(heads)::value;
+                Raw8 raw[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    raw[e] = Raw8{*reinterpret_cast<const uint2 *>(from_a + e * D), *reinterpret_cast<const uint2 *>(from_b + e * D)};
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    float x[8];
+                    decode8<HALF>(raw[e], x);
+                    turn8<MODE>(x, t, at_k, p.paired);
+                    *reinterpret_cast<uint2 *>(to_a + e * D) = make_uint2(pack16<HALF>(x[0], x[1]), pack16<HALF>(x[2], x[3]));
+                    *reinterpret_cast<uint2 *>(to_b + e * D) = make_uint2(pack16<HALF>(x[4], x[5]), pack16<HALF>(x[6], x[7]));
+                }
+                from_a += N * D, from_b += N * D, to_a += N * D, to_b += N * D;
+            };
+            int left = group;
+#pragma unroll 1
+            for (; left >= kHeads; left -= kHeads) some(std::integral_constant<int, kHeads>());
+#pragma unroll 1
+            for (; left > 0; --left) some(std::integral_constant<int, 1>());
+        };
+        if (page < 0)
+            for (int row = r0; row < count; row += kRows) queries(row, angles_of(p, pos0 + row, i, at_k.turned));
         if (page >= 0) {
             const size_t block = (size_t)page * p.kv_heads + h;
             const float old_k = begin ? p.k_scale[block] : 0.f, old_v = begin ? p.v_scale[block] : 0.f;
-            float k[R][8];
-            Raw8 v[R];
             unsigned mk = 0, mv = 0;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int row = r0 + r * kRows;
-                if (row < count) {
-                    v[r] = fetch8(p.v + (token0 + row) * p.v_ld + h * D, at_v);
-                    const Angles t = angles_of(p, pos0 + row, i, at_k.turned);
-                    decode8<HALF>(fetch8(p.k + (token0 + row) * p.k_ld + h * D, at_k), k[r]);
-                    if (at_k.turned) turn8(k[r], t, p.paired);
-                    mk = max(mk, amax8(k[r]));
-                }
+            bool wild = false;
+#pragma unroll 1
+            for (int row = r0; row < count; row += kRows) {
+                const Raw8 v = fetch8(p.v + (token0 + row) * p.v_ld + h * D, at_v);
+                const Angles t = angles_of(p, pos0 + row, i, at_k.turned);
+                const Raw8 k = fetch8(p.k + (token0 + row) * p.k_ld + h * D, at_k);
+                queries(row, t);
+                float x[8];
+                decode8<HALF>(k, x);
+                turn8<MODE>(x, t, at_k, p.paired);
+                mk = max(mk, amax8(x, wild));
+                float4 *at = keys + row * (D / 4) + i;  // (sixteen bytes a lane, twice: no two lanes of a phase in a bank)
+                at[0] = make_float4(x[0], x[1], x[2], x[3]), at[kLanes] = make_float4(x[4], x[5], x[6], x[7]);
+                values[row * kLanes + i] = make_uint4(v.a.x, v.a.y, v.b.x, v.b.y);
+                decode8<HALF>(v, x);
+                mv = max(mv, amax8(x, wild));
             }
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (r0 + r * kRows < count) {
-                    float x[8];
-                    decode8<HALF>(v[r], x);
-                    mv = max(mv, amax8(x));
-                }
             mk = __reduce_max_sync(0xffffffffu, mk), mv = __reduce_max_sync(0xffffffffu, mv);
             if ((threadIdx.x & 31) == 0) atomicMax(&s_amax[0], mk), atomicMax(&s_amax[1], mv);
             __syncthreads();
             const float scale_k = fmaxf(old_k, scale_for(s_amax[0])), scale_v = fmaxf(old_v, scale_for(s_amax[1]));
             const float inv_k = 1.0f / scale_k, inv_v = 1.0f / scale_v;
             unsigned char *to_k = p.k_codes + block * page_tokens * D, *to_v = p.v_codes + block * page_tokens * D;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int row = r0 + r * kRows;
-                if (row < count) {
-                    store8(to_k + (begin + row) * D, at_k, k[r], inv_k);
-                    float x[8];
-                    decode8<HALF>(v[r], x);
-                    store8(to_v + (begin + row) * D, at_v, x, inv_v);
-                }
+#pragma unroll 2
+            for (int row = r0; row < count; row += kRows) {
+                const float4 *at = keys + row * (D / 4) + i;
+                const float4 a = at[0], b = at[kLanes];
+                const uint4 v = values[row * kLanes + i];
+                float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                store8(to_k + (begin + row) * D, at_k, x, inv_k, wild);
+                decode8<HALF>(Raw8{make_uint2(v.x, v.y), make_uint2(v.z, v.w)}, x);
+                store8(to_v + (begin + row) * D, at_v, x, inv_v, wild);
             }
             if (scale_k > old_k && begin)
                 for (int e = threadIdx.x; e < begin * (D / 4); e += kAppendThreads) {
@@ -313,43 +365,31 @@ kv_append_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
                 }
             if (threadIdx.x == 0) p.k_scale[block] = scale_k, p.v_scale[block] = scale_v;
         }
-        // the group's queries
-        for (int e = r0; e < count * group; e += kRows) {
-            const int row = e / group, head = h * group + e % group;
-            const Angles t = angles_of(p, pos0 + row, i, at_k.turned);
-            float x[8];
-            decode8<HALF>(fetch8(p.q + (token0 + row) * p.q_ld + head * D, at_k), x);
-            if (at_k.turned) turn8(x, t, p.paired);
-            unsigned short *out = p.q_out + (token0 + row) * p.q_out_ld + head * D;
-            *reinterpret_cast<uint2 *>(out + at_k.a) = make_uint2(pack16<HALF>(x[0], x[1]), pack16<HALF>(x[2], x[3]));
-            *reinterpret_cast<uint2 *>(out + at_k.b) = make_uint2(pack16<HALF>(x[4], x[5]), pack16<HALF>(x[6], x[7]));
-        }
         __syncthreads();  // the tile number and the amaxes are rewritten
     }
     if (threadIdx.x == 0) trace_end(blp, iter);
 }
 
 template <typename F>
-static auto append_instance(int dim, bool half, int page_tokens, F &&f) {
-    auto rows = [&](auto d, auto hf) {
+static auto append_instance(int dim, bool half, int mode, F &&f) {
+    auto modes = [&](auto d, auto hf) {
         constexpr int D = decltype(d)::value;
         constexpr bool H = decltype(hf)::value;
-        switch (page_tokens / (kAppendThreads / (D / 8))) {
-            case 0:
-            case 1: return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, 1, H>);
-            case 2: return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, 2, H>);
-            case 4: return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, 4, H>);
-            default: return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, 8, H>);
-        }
+        if (mode == TURN_HALVES) return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, H, TURN_HALVES>);
+        if (mode == TURN_PAIRS) return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, H, TURN_PAIRS>);
+        return f(kv_append_one_kernel<D, H>, kv_append_kernel<D, H, TURN_ANY>);
     };
-    if (dim == 64) return half ? rows(std::integral_constant<int, 64>(), std::true_type()) : rows(std::integral_constant<int, 64>(), std::false_type());
-    return half ? rows(std::integral_constant<int, 128>(), std::true_type()) : rows(std::integral_constant<int, 128>(), std::false_type());
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    if (dim == 64) return half ? modes(D64(), std::true_type()) : modes(D64(), std::false_type());
+    return half ? modes(D128(), std::true_type()) : modes(D128(), std::false_type());
 }
 
 static cudaError_t append_launch(const AppendParams &p, int dim, bool half, const DeviceInfo &d, BlpArgs blp, cudaStream_t s) {
     const int sm_count = d.sm_count, device = d.device;
     const int page_tokens = 1 << p.page_shift;
-    return append_instance(dim, half, page_tokens, [&](auto one, auto any) {
+    const int mode = p.rotated != dim ? TURN_ANY : p.paired ? TURN_PAIRS : TURN_HALVES;
+    return append_instance(dim, half, mode, [&](auto one, auto any) {
         int per_sm;
         if (p.batch.most_new == 1) {
             const long long rows = (long long)p.batch.seqs * (2 * p.kv_heads + (p.q ? p.heads : 0));
@@ -360,7 +400,7 @@ static cudaError_t append_launch(const AppendParams &p, int dim, bool half, cons
             const int grid = (int)std::min<long long>(blp.total_tiles, (long long)sm_count * per_sm);
             return launch_layer(one, grid, kAppendOneThreads, 0, s, p, blp);
         }
-        const size_t smem = (p.batch.seqs + 1) * sizeof(int);
+        const size_t smem = (size_t)page_tokens * dim * 6 + (p.batch.seqs + 1) * sizeof(int);
         const cudaError_t e = lm_resident((const void *)any, kAppendThreads, smem, device, &per_sm);
         if (e != cudaSuccess) return e;
         // (pages that new tokens can touch: full ones, and two parts of one a sequence)
