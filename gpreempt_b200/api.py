@@ -303,11 +303,11 @@ def gemm_tiles(m: int, n: int) -> int:
 
 def _address(x) -> int | None:
     """Device address of a DeviceBuffer, an array with data_ptr() or an integer; None stays None."""
-    if x is None or isinstance(x, int):
+    if x is None or type(x) is int:
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
-    return x.ptr.value
+    if type(x) is DeviceBuffer:
+        return x.ptr.value
+    return x.data_ptr()
 
 
 class LmContext(_Resettable):

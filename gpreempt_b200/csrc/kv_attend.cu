@@ -115,8 +115,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     int tiles = dynamic ? max((n_line + p.blocks_a_tile - 1) / p.blocks_a_tile, (int)gridDim.x) : (int)gridDim.x;
     tiles = min(min(tiles, n_line), p.max_tiles);
     blp.total_tiles = tiles;
-    auto tile_begin = [&](int t) { return (int)((long long)t * n_line / tiles); };
-    auto tile_of = [&](int b) { return (int)((((long long)b + 1) * tiles - 1) / n_line); };
+    const LmCut cut(n_line, tiles);
     auto wait = [&](unsigned long long *bar, uint32_t phase) {
         if (!mbar_wait(smem_u32(bar), phase, abort_flag, kAttWaitNs)) {
             *abort_flag = 1;
@@ -154,7 +153,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             tile = blp_claim(blp, iter);
         }
         if (tile < 0) break;
-        const int line0 = tile_begin(tile), line1 = tile_begin(tile + 1);
+        const int line0 = cut.begin(tile), line1 = cut.begin(tile + 1);
 
         if (wid == kAttWarps) {
             // ---- the ring's filler
@@ -167,13 +166,13 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     const int mine = lane / pieces, sub = lane - mine * pieces;
                     const int key = u.key0 + (block0 + b0 + mine) * kAttKeys + sub * per_page;
                     int row = -1;
-                    float ks = 1.f, vs = 0.f;
+                    float ks = 1.f, vs = 1.f;
                     if (b0 + mine < blocks_live && key < u.high) {
                         const int page = p.batch.table[(size_t)u.s * p.batch.table_ld + (key >> p.page_shift)];
                         if ((unsigned)page < (unsigned)p.pages) {
                             const long long block = (long long)page * p.kv_heads + u.head;
                             row = (int)((block << p.page_shift) + (key & (page_tokens - 1)));
-                            ks = p.k_scale[block], vs = log2f(fmaxf(p.v_scale[block], 1.17549435e-38f));
+                            ks = p.k_scale[block], vs = p.v_scale[block];
                         } else {
                             lm_fail(p.error, LM_BAD_PAGE, u.s);
                         }
@@ -182,20 +181,20 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     for (int b = 0; b < some; ++b) {
                         wait(&ctl->empty[stage], phase ^ 1);
                         const bool loads = mine == b && row >= 0;
-                        if (mine == b) {
-                            for (int w = sub * per_page / 16; w < (sub + 1) * per_page / 16; ++w)
-                                ctl->scales[stage][w][0] = ks, ctl->scales[stage][w][1] = vs;
-                        }
-                        const int loading = __popc(__ballot_sync(0xffffffffu, loads));
-                        __syncwarp();  // the scales are written before the stage is announced
                         const uint32_t full = smem_u32(&ctl->full[stage]);
-                        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(loading * 2 * per_page * D));
-                        __syncwarp();
                         if (loads) {
+                            // (ahead of the stage's arrival, which waits for the scales: it cannot complete before)
                             const uint32_t at = ring + stage * 2 * Cfg::kTile + sub * per_page * D;
                             tma_load_2d(at, &p.map_k, full, 0, row);
                             tma_load_2d(at + Cfg::kTile, &p.map_v, full, 0, row);
                         }
+                        if (mine == b) {
+                            for (int w = sub * per_page / 16; w < (sub + 1) * per_page / 16; ++w)
+                                ctl->scales[stage][w][0] = ks, ctl->scales[stage][w][1] = log2f(fmaxf(vs, 1.17549435e-38f));
+                        }
+                        const int loading = __popc(__ballot_sync(0xffffffffu, loads));
+                        __syncwarp();  // the scales are written before the stage is announced
+                        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(loading * 2 * per_page * D));
                         __syncwarp();
                         advance();
                     }
@@ -207,6 +206,8 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kAttConsumers) : "memory"); };
             each_piece(line0, line1, [&](const Unit &u, int block0, int blocks, int unit0, int unit_blocks) {
                 const int blocks_live = min(blocks, max(0, (u.high - u.key0 + kAttKeys - 1) / kAttKeys - block0));
+                const bool whole = blocks == unit_blocks;
+                const int t0 = whole ? tile : cut.tile_of(unit0), t1 = whole ? tile : cut.tile_of(unit0 + unit_blocks - 1);
                 // ---- the unit's queries as operands: warp w prepares tiles of eight rows w, w + 4, ...
                 for (int nt = wid; nt < NT; nt += kAttWarps) {
                     const int r = nt * 8 + g;
@@ -538,7 +539,6 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     const int at = u.row0 + r;
                     return p.lse + (long long)(u.first + at / group) * p.heads + u.head * group + at % group;
                 };
-                const bool whole = blocks == unit_blocks;
                 constexpr int kSlot = ROWS * (D + 2);  // floats: maxima, sums, outputs
                 if (wid == 0) {
 #pragma unroll
@@ -572,7 +572,6 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                             }
                         }
                     if (!whole) {
-                        const int t0 = tile_of(unit0), t1 = tile_of(unit0 + unit_blocks - 1);
                         __threadfence();
                         __syncwarp();
                         if (lane == 0) ctl->last = atomicAdd(&p.counters[t0], 1) == t1 - t0;
@@ -586,8 +585,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 if (ctl->last) {
                     // ---- join the parts in the order of the line: a warp a row, a lane D / 32 elements
                     __threadfence();
-                    const int t0 = tile_of(unit0), t1 = tile_of(unit0 + unit_blocks - 1);
-                    const int slot0 = 2 * t0 + (unit0 > tile_begin(t0) ? 1 : 0);
+                    const int slot0 = 2 * t0 + (unit0 > cut.begin(t0) ? 1 : 0);
                     auto slot_of = [&](int x) { return p.parts + (size_t)(x == t0 ? slot0 : 2 * x) * kSlot; };
                     for (int r = wid; r < u.rows; r += kAttWarps) {
                         float mm = -INFINITY;

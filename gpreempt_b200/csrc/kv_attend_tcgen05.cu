@@ -56,6 +56,8 @@ struct ManyCfg {
     static constexpr int kSlot = 2 * kTileRows + kTileRows * D;  // floats: maxima, sums, outputs [D / 4][row][4]
 };
 
+constexpr int kFewSeqs = 128;
+
 struct ManyCtl {
     unsigned long long raw_full[kRawStages], raw_empty[kRawStages];
     unsigned long long keys_full[kKeyBuffers], keys_empty[kKeyBuffers];
@@ -68,6 +70,7 @@ struct ManyCtl {
     int end;                  // the block of the unit at which the piece ends
     int stopped;              // because of the word
     int saw_nan, last, longest, abort_flag;
+    int prefix[kFewSeqs];
 };
 
 // The largest of three (one instruction on this architecture).
@@ -97,7 +100,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     ManyCtl *ctl = reinterpret_cast<ManyCtl *>(smem + Cfg::kCtlAt);
-    int *const prefix = p.prefix;  // [seqs + 1], the same from every CTA (shared memory is full)
+    // [seqs + 1]; of many sequences in the context, the same from every CTA (shared memory is full)
+    int *const prefix = p.batch.seqs < kFewSeqs ? ctl->prefix : p.prefix;
     volatile int *abort_flag = &ctl->abort_flag;
     const uint32_t base = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, wid = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -174,8 +178,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     const int tiles = by_unit ? n_line : min(n_line, (int)gridDim.x);
     blp.total_tiles = tiles;
     auto on_line = [&](const Unit &u) { return by_unit ? 1 : blocks_of(u); };  // what a unit takes of the line
-    auto tile_begin = [&](int t) { return (int)((long long)t * n_line / tiles); };
-    auto tile_of = [&](int b) { return (int)((((long long)b + 1) * tiles - 1) / n_line); };
+    const LmCut cut(n_line, tiles);
     int *const note = p.counters + kLmCounters - kNotes + 4 * blockIdx.x;
     float *const spill = p.parts + (size_t)(p.max_tiles - (int)gridDim.x + (int)blockIdx.x) * Cfg::kSlot;
     auto largest_scale = [&]() { return fmaxf(fmaxf(fmaxf(ctl->largest[0], ctl->largest[1]), fmaxf(ctl->largest[2], ctl->largest[3])), 1.17549435e-38f); };
@@ -210,8 +213,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             Piece x;
             x.tile = ctl->tile;
             if (x.tile < 0) return;
-            x.line0 = tile_begin(x.tile);
-            const int line1 = tile_begin(x.tile + 1);
+            x.line0 = cut.begin(x.tile);
+            const int line1 = cut.begin(x.tile + 1);
             // the first unit: its sequence, head and block of rows
             // (where a unit is a tile, its place on the line is not that of its blocks: what is done of it is added below)
             int at = x.line0 + (by_unit ? 0 : ctl->done);
@@ -261,7 +264,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     return;
                 }
                 if (!x.whole) {
-                    const int t0 = tile_of(x.unit0), t1 = tile_of(x.unit0 + x.unit_blocks - 1);
+                    const int t0 = cut.tile_of(x.unit0), t1 = cut.tile_of(x.unit0 + x.unit_blocks - 1);
                     if (tid == 0) {
                         __threadfence();
                         ctl->last = atomicAdd(&p.counters[t0], 1) == t1 - t0;
@@ -338,14 +341,14 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 for (int i = 0; i < 2; ++i) {
                     const int st = n_raw % kRawStages;
                     wait(&ctl->raw_empty[st], (n_raw / kRawStages & 1) ^ 1);
+                    const uint32_t full = smem_u32(&ctl->raw_full[st]);
+                    // (ahead of the stage's arrival, which waits for the scales: it cannot complete before)
+                    if (loads) tma_load_2d(base + Cfg::kRawAt + st * Cfg::kCodes + sub * per_page * D, i ? &p.map_v : &p.map_k, full, 0, row);
                     if (i == 0 && mine == b)
                         for (int w = sub * per_page / 16; w < (sub + 1) * per_page / 16; ++w)
                             ctl->scales[(j + b) & 3][w][0] = ks, ctl->scales[(j + b) & 3][w][1] = vs;
                     __syncwarp();
-                    const uint32_t full = smem_u32(&ctl->raw_full[st]);
                     if (lane == 0) mbar_arrive_expect_tx(full, bytes);
-                    __syncwarp();
-                    if (loads) tma_load_2d(base + Cfg::kRawAt + st * Cfg::kCodes + sub * per_page * D, i ? &p.map_v : &p.map_k, full, 0, row);
                     __syncwarp();
                     ++n_raw;
                 }
@@ -772,7 +775,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         const int row_at = u.row0 + r;
         const long long token = u.first + row_at / group;
         const int q_head = u.head * group + row_at % group;
-        const int slot0 = 2 * t0 + (x.unit0 > tile_begin(t0) ? 1 : 0), parts = t1 - t0 + 1;
+        const int slot0 = 2 * t0 + (x.unit0 > cut.begin(t0) ? 1 : 0), parts = t1 - t0 + 1;
         auto slot_of = [&](int q) { return p.parts + (size_t)(q == 0 ? slot0 : 2 * (t0 + q)) * Cfg::kSlot; };
         float m = -INFINITY, l = 0.f;
         for (int q = 0; q < parts; ++q) m = fmaxf(m, __ldcg(slot_of(q) + r));
