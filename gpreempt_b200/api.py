@@ -9,6 +9,7 @@ the GPU through libgpx; nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
@@ -301,13 +302,39 @@ def gemm_tiles(m: int, n: int) -> int:
 # ---- serving a decoder -------------------------------------------------------------------------
 
 
-def _address(x) -> int | None:
-    """Device address of a DeviceBuffer, an array with data_ptr() or an integer; None stays None."""
-    if x is None or type(x) is int:
+def _address(x) -> int:
+    """Device address of a DeviceBuffer, an array with data_ptr() or an integer; 0 for None."""
+    if type(x) is int:
         return x
+    if x is None:
+        return 0
     if type(x) is DeviceBuffer:
         return x.ptr.value
     return x.data_ptr()
+
+
+# The argument structures of include/gpx.h as packed bytes: a ctypes structure of fifteen fields takes 2 us to fill, which a
+# launch of 4 us notices.
+_APPEND_ARGS, _ATTEND_ARGS, _SCORES_ARGS = struct.Struct("6Q4q4iQ"), struct.Struct("3Q2q3ifQ"), struct.Struct("7Qq3ifQ")
+_dtype_names: dict = {}
+
+
+def _dtype(name: str) -> int:
+    """Address of a dtype's name, kept for the process."""
+    known = _dtype_names.get(name)
+    if known is None:
+        text = ctypes.create_string_buffer(name.encode())
+        known = _dtype_names[name] = (ctypes.addressof(text), text)
+    return known[0]
+
+
+def _lm_call(entry, ctx, blp, stream, *arguments) -> None:
+    h = _h(stream) if stream is not None else None
+    if ctx._pending:
+        ctx.order(h)
+    status = entry(*arguments, ctx._buf.ptr, _blp_for(blp, h) if blp is not None else None, h)
+    if status != B.SUCC:
+        check(status)
 
 
 class LmContext(_Resettable):
@@ -384,34 +411,28 @@ class Rope:
 def kv_append(cache: KvCache, batch: KvBatch, q, k, v, q_out, heads: int, dtype: str, ctx: LmContext, rope: Rope | None = None,
               blp: BlpContext | None = None, stream=None, q_ld: int = 0, k_ld: int = 0, v_ld: int = 0, q_out_ld: int = 0) -> None:
     """Appends a step's keys and values to the cache; turns queries (q to q_out, or both None) and keys on the way."""
-    h = _h(stream)
-    ctx.order(h)
-    turn = (rope.cos, rope.sin, rope.rotated, rope.positions, rope.paired) if rope is not None else (None, None, 0, 0, 0)
-    args = B.KvAppendArgs(_address(q), _address(k), _address(v), _address(q_out), turn[0], turn[1], q_ld, k_ld, v_ld, q_out_ld, heads,
-                          turn[2], turn[3], turn[4], dtype.encode())
-    check(B.load().gpx_kv_append(cache.handle, batch._ref, ctypes.byref(args), ctx._buf.ptr, _blp_for(blp, h), h))
+    turn = (rope.cos, rope.sin) if rope is not None else (0, 0)
+    how = (rope.rotated, rope.positions, rope.paired) if rope is not None else (0, 0, 0)
+    args = _APPEND_ARGS.pack(_address(q), _address(k), _address(v), _address(q_out), *turn, q_ld, k_ld, v_ld, q_out_ld, heads, *how, _dtype(dtype))
+    _lm_call(B.load().gpx_kv_append, ctx, blp, stream, cache.handle, batch._ref, args)
 
 
 def kv_attend(cache: KvCache, batch: KvBatch, q, out, heads: int, dtype: str, ctx: LmContext, scale: float = 0.0, causal: bool = True,
               window: int = 0, lse=None, blp: BlpContext | None = None, stream=None, q_ld: int = 0, out_ld: int = 0) -> None:
     """Attention of a step's new tokens over their sequences' pages (scale 0: 1 / sqrt(head_dim))."""
-    h = _h(stream)
-    ctx.order(h)
-    args = B.KvAttendArgs(_address(q), _address(out), _address(lse), q_ld, out_ld, heads, int(causal), window, scale, dtype.encode())
-    check(B.load().gpx_kv_attend(cache.handle, batch._ref, ctypes.byref(args), ctx._buf.ptr, _blp_for(blp, h), h))
+    args = _ATTEND_ARGS.pack(_address(q), _address(out), _address(lse), q_ld, out_ld, heads, int(causal), window, scale, _dtype(dtype))
+    _lm_call(B.load().gpx_kv_attend, ctx, blp, stream, cache.handle, batch._ref, args)
 
 
 def token_scores(logits, rows: int, vocab: int, dtype: str, ctx: LmContext, targets=None, logprob=None, entropy=None, lse=None,
                  top: int = 0, top_ids=None, top_logprob=None, temperature: float = 1.0, ld: int = 0, blp: BlpContext | None = None,
                  stream=None) -> None:
     """Log probabilities of `targets`, entropies and the `top` most likely tokens of each row of logits."""
-    h = _h(stream)
-    ctx.order(h)
     if not top:  # (arrays of no elements have no address worth passing)
         top_ids = top_logprob = None
-    args = B.TokenScoresArgs(_address(logits), _address(targets), _address(logprob), _address(entropy), _address(lse), _address(top_ids),
-                             _address(top_logprob), ld, rows, vocab, top, 1.0 / temperature if temperature else 0.0, dtype.encode())
-    check(B.load().gpx_token_scores(ctypes.byref(args), ctx._buf.ptr, _blp_for(blp, h), h))
+    args = _SCORES_ARGS.pack(_address(logits), _address(targets), _address(logprob), _address(entropy), _address(lse), _address(top_ids),
+                             _address(top_logprob), ld, rows, vocab, top, 1.0 / temperature if temperature else 0.0, _dtype(dtype))
+    _lm_call(B.load().gpx_token_scores, ctx, blp, stream, args)
 
 
 def synth_normal(n: int, seed: int, stream: int = 0, mean: float = 0.0, std: float = 1.0):

@@ -152,9 +152,9 @@ _SIGS = {
     "gpx_lm_status": [vp, P(ci), P(ci)],
     "gpx_kv_cache_create": [vp, vp, vp, vp, ci, ci, ci, ci, P(vp)],
     "gpx_kv_cache_destroy": [vp],
-    "gpx_kv_append": [vp, P(KvBatch), P(KvAppendArgs), vp, P(Blp), vp],
-    "gpx_kv_attend": [vp, P(KvBatch), P(KvAttendArgs), vp, P(Blp), vp],
-    "gpx_token_scores": [P(TokenScoresArgs), vp, P(Blp), vp],
+    "gpx_kv_append": [vp, vp, vp, vp, vp, vp],  # (structures by address: packed bytes, or ctypes.byref)
+    "gpx_kv_attend": [vp, vp, vp, vp, vp, vp],
+    "gpx_token_scores": [vp, vp, vp, vp],
     "gpx_synth_normal": [vp, sz, u64, u64, ctypes.c_float, ctypes.c_float],
     "gpx_synth_uniform": [vp, sz, u64, u64, ctypes.c_float, ctypes.c_float],
     "gpx_model_open": [ctypes.c_char_p, P(ModelOpts), P(vp)],

@@ -87,3 +87,18 @@ def test_score_refusals(lib):
     word = B.Blp(preempted=p)
     a = B.TokenScoresArgs(logits=p, rows=2, vocab=100, inv_temperature=1.0, dtype=b"float32")
     assert lib.gpx_token_scores(ctypes.byref(a), ctx, ctypes.byref(word), None) == B.FAIL and b"stop_index" in lib.gpx_last_error()
+
+
+def test_packed_arguments_have_the_structures_layout():
+    from gpreempt_b200 import api
+
+    for packed, structure in ((api._APPEND_ARGS, B.KvAppendArgs), (api._ATTEND_ARGS, B.KvAttendArgs), (api._SCORES_ARGS, B.TokenScoresArgs)):
+        assert packed.size == ctypes.sizeof(structure)
+        values = tuple(range(1, 1 + len(structure._fields_)))
+        raw = structure.from_buffer_copy(packed.pack(*values))
+        for value, (name, kind) in zip(values, structure._fields_):
+            if kind is ctypes.c_char_p:  # (an address that is not to be followed)
+                at = getattr(structure, name).offset
+                assert int.from_bytes(bytes(raw)[at:at + 8], "little") == value
+            else:
+                assert getattr(raw, name) == value
