@@ -634,7 +634,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             };
             uint32_t h[64];
             float sum, plain;  // of the factors as the normaliser and as the operand has them
-            auto exponentials = [&](auto masked) {
+            // careful: keys may be masked, and the exponents are rounded as largest() rounds them before the reference is taken off
+            auto exponentials = [&](auto careful) {
                 const float ref = m == -INFINITY ? 0.f : m;
                 sum = plain = 0.f;
                 uint32_t both[2][32];
@@ -650,14 +651,16 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                         tmem_ld_32x32(t_s + 32 * (c + 1), both[(c + 1) & 1]);
                         next[0] = of[2 * c + 2], next[1] = of[2 * c + 3];
                     }
-                    if (decltype(masked)::value) hide(c, v);
+                    if (decltype(careful)::value) hide(c, v);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        const float2 by = make_float2(g[q].x * mult, g[q].x * mult), plus = make_float2(g[q].z - ref, g[q].z - ref);
+                        const float less = decltype(careful)::value ? g[q].z : g[q].z - ref;
+                        const float2 by = make_float2(g[q].x * mult, g[q].x * mult), plus = make_float2(less, less);
                         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                         for (int i = 8 * q; i < 8 * q + 8; ++i) {
-                            const float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, plus);
+                            float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, plus);
+                            if (decltype(careful)::value) y.x -= ref, y.y -= ref;
                             const float2 e = make_float2(lm_ex2(y.x), lm_ex2(y.y));
                             part[i & 1] = add2(part[i & 1], e);
                             h[16 * c + i] = pack_halves(e.x, e.y);
@@ -673,10 +676,14 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 const float most = largest();
                 if (m == -INFINITY) m = most;
             }
-            for (bool again = masks;; again = true) {
-                if (again) exponentials(std::true_type());
+            // (Exponents of 2^20 and more are rounded first throughout: one sum with the reference would leave the largest off 0 by
+            // up to 2^-24 of itself, which can be more than the range of a half.  So it is where the pass is repeated.)
+            const bool large = __any_sync(0xffffffffu, fabsf(m) > 1048576.f && m != -INFINITY);
+            for (int pass = 0;; ++pass) {
+                if (pass || masks || large) exponentials(std::true_type());
                 else exponentials(std::false_type());
-                if (!__any_sync(0xffffffffu, plain > kMostFactors)) break;
+                // (once is enough, unless a page's scale is not positive, which is no reason to go on without end)
+                if (pass || !__any_sync(0xffffffffu, plain > kMostFactors)) break;
                 // (the scores' arrival means that the products before them are complete)
                 const float now = fmaxf(m, largest()), f = now == -INFINITY ? 1.f : lm_ex2(m - now);
 #pragma unroll 1

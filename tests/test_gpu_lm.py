@@ -339,6 +339,27 @@ def test_rows_that_one_key_dominates(gpx, ctx):
         bed.free()
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("power", [6, 24, 30, 60, 100])
+def test_scores_of_any_magnitude(gpx, ctx, new, power):
+    """One key ahead of all others by 2^power and more: it alone counts, whatever the rounding of such scores."""
+    c, heads, kv, dim, page = 700, 2, 1, 128, 64
+    q = np.zeros((new, heads, dim), np.float32)
+    q[:, :, 0] = 2.0 ** power
+    for at, scale in ((0, 1.0), (333, 0.75), (340, 1.0 / 3), (699, 1.3)):
+        bed = Bed(gpx, [new], [c], heads, kv, dim, page, seed=at)
+        bed.k[..., 0] = bed.rng.integers(0, 0x7D, bed.k[..., 0].shape)  # 384 at most
+        bed.k[bed.table[0, at // page], 0, at % page, 0] = 0x7E  # 448
+        bed.ks[:] = 1.0
+        bed.upload()
+        got, lse = run_attention(gpx, ctx, bed, q, "bfloat16", heads, causal=False, scale=scale)
+        v = lm.decode(bed.v[bed.table[0, at // page], 0, at % page]) * bed.vs[bed.table[0, at // page], 0]
+        assert np.array_equal(got, np.broadcast_to(from_bits(to_bits(v.astype(np.float32), "bfloat16"), "bfloat16"), got.shape))
+        want = 448.0 * 2.0 ** power * float(np.float32(scale))
+        assert np.all(np.abs(lse - want) <= 2.0 ** -20 * want)
+        bed.free()
+
+
 def test_cache_beyond_four_gigabytes(gpx, ctx):
     """Pages whose bytes lie past 32 bits; the pool is not initialised elsewhere."""
     pages, page, kv, dim, heads = 36000, 128, 8, 128, 16  # 4.7 GB of keys, as many of values
