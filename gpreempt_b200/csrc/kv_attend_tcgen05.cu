@@ -80,6 +80,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
+__device__ __forceinline__ void st_shared_v4(uint32_t to, const uint4 &v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t from) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+    return v;
+}
+
+// A warp's rows in the layout of an operand, as many lanes a row as it has pieces of 16 bytes: of a step i, a lane has `piece` of
+// row first + i.  (A thread a row, as the scores are, has as many lines in an access as lanes.)
+template <int D>
+struct WarpRows {
+    static constexpr int kLanes = D / 8;
+    int piece, first;
+    uint32_t base;
+    __device__ __forceinline__ WarpRows(uint32_t operand, int wid, int lane) {
+        piece = lane % kLanes, first = lane / kLanes * kLanes;
+        base = operand + (piece >> 3) * (128 * 128) + ((wid & 3) * 32 + first) * 128;
+    }
+    __device__ __forceinline__ uint32_t in_operand(int i) const { return base + i * 128 + (((piece ^ i) & 7) << 4); }
+};
+
 // A piece of a unit that a tile has.
 struct Piece {
     Unit u;
@@ -96,6 +119,7 @@ template <int D, bool HALF>
 __global__ void __launch_bounds__(kManyThreads, 1)
 kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     using Cfg = ManyCfg<D>;
+    using Rows = WarpRows<D>;
     constexpr uint32_t kHalfTile = 128 * 128;  // bytes of 128 rows of 64 halves
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -542,11 +566,24 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         float factor = 1.f;
         {
             // the row's queries, as halves, into the swizzled operand
-            const uint4 *q = reinterpret_cast<const uint4 *>(p.q + token * p.q_ld + (long long)q_head * D);
             unsigned char *to = smem + w * Cfg::kQ + row * 128;
             uint4 v[D / 8];
+            {
+                const Rows at(base + w * Cfg::kQ, wid, lane);
+                const long long own = token * p.q_ld + (long long)q_head * D;  // (rows past the last have its queries: a condition would make one load wait for another)
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) v[c] = live ? q[c] : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < Rows::kLanes; ++i) {
+                    const long long from = __shfl_sync(0xffffffffu, own, at.first + i);
+                    v[i] = reinterpret_cast<const uint4 *>(p.q + from)[at.piece];
+                }
+#pragma unroll
+                for (int i = 0; i < Rows::kLanes; ++i) st_shared_v4(at.in_operand(i), v[i]);
+                __syncwarp();
+            }
+            if (!HALF) {
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) v[c] = *reinterpret_cast<const uint4 *>(to + (c >> 3) * kHalfTile + (((c & 7) ^ (row & 7)) << 4));
+            }
             float inv = 1.f;
             if (!HALF) {
                 uint32_t most = 0;
@@ -561,14 +598,11 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 inv = 1.0f / factor;
             }
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                if (!HALF) {
-                    uint32_t e[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+            for (int c = 0; !HALF && c < D / 8; ++c) {
+                uint32_t e[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[i] = pack_halves(__uint_as_float(e[i] << 16) * inv, __uint_as_float(e[i] & 0xffff0000u) * inv);
-                    v[c] = make_uint4(e[0], e[1], e[2], e[3]);
-                }
-                *reinterpret_cast<uint4 *>(to + (c >> 3) * kHalfTile + (((c & 7) ^ (row & 7)) << 4)) = v[c];
+                for (int i = 0; i < 4; ++i) e[i] = pack_halves(__uint_as_float(e[i] << 16) * inv, __uint_as_float(e[i] & 0xffff0000u) * inv);
+                *reinterpret_cast<uint4 *>(to + (c >> 3) * kHalfTile + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
             }
         }
         const float mult = factor * p.scale * 1.4426950408889634f;
@@ -736,7 +770,6 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         // (a row without keys is zero; one whose keys all score -infinity is not a number, as the formula says)
         const bool empty = hi <= 0;
         const float inv = empty ? 0.f : unit / l;
-        uint32_t *out = reinterpret_cast<uint32_t *>(p.out + token * p.out_ld + (long long)q_head * D);
 #pragma unroll
         for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
@@ -756,13 +789,27 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 for (int i = 0; i < 4; ++i)
                     to[(c / 4 + i) * kTileRows] = make_float4(__uint_as_float(o[4 * i]) * f, __uint_as_float(o[4 * i + 1]) * f,
                                                               __uint_as_float(o[4 * i + 2]) * f, __uint_as_float(o[4 * i + 3]) * f);
-            } else if (live) {
+            } else {
+                // (to where the queries were, which no product reads any more)
                 uint32_t h[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     h[i] = empty ? 0u : pack_out<HALF>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-                reinterpret_cast<uint4 *>(out + c / 2)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-                reinterpret_cast<uint4 *>(out + c / 2)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+                unsigned char *to = smem + w * Cfg::kQ + (c >> 6) * kHalfTile + row * 128;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<uint4 *>(to + (((c / 8 + i) & 7) ^ (row & 7)) * 16) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+            }
+        }
+        if (!to_context) {
+            __syncwarp();
+            const Rows at(base + w * Cfg::kQ, wid, lane);
+            const long long own = live ? token * p.out_ld + (long long)q_head * D : -1;
+#pragma unroll
+            for (int i = 0; i < Rows::kLanes; ++i) {
+                const long long to = __shfl_sync(0xffffffffu, own, at.first + i);
+                const uint4 v = ld_shared_v4(at.in_operand(i));
+                if (to >= 0) reinterpret_cast<uint4 *>(p.out + to)[at.piece] = v;
             }
         }
         if (to_context) {
