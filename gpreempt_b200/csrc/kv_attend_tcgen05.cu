@@ -42,6 +42,9 @@ constexpr unsigned long long kManyWaitNs = 2000000000ull;
 // half holds; then the maximum is taken anew and the sums are rescaled.  (Asking for the maximum of every block goes
 // through its scores twice, and a new one among 32 rows, which are rescaled together, comes in most blocks.)
 constexpr float kMostFactors = 32768.f;
+// What the start of a unit takes (queries, the first blocks until their products run, outputs), in blocks: that many places of the
+// line come before its own, so that a tile of many short units has as long as one of a single long unit.
+constexpr int kUnitCost = 8;
 // Blocks of the longest unit up to which units are not cut.
 constexpr int kShortUnit = 8;
 constexpr int kNotes = 1024;  // the last counters of the context: {tile + 1, blocks done, whether sums were left} of a CTA's unfinished tile
@@ -173,7 +176,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         for (int i = 0; all >= 0 && i < rows; ++i) {
             const int blocks = blocks_of(lay.unit(s, i));
             if (blocks > kShortUnit) ctl->longest = blocks;
-            all += blocks;
+            all += blocks + kUnitCost;
         }
         count[s] = (int)min(all < 0 ? all : all * p.kv_heads, 0x7fffffffll);
     }
@@ -185,7 +188,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         for (int i = lane; i < rows; i += 32) {
             const int blocks = blocks_of(lay.unit(s, i));
             if (blocks > kShortUnit) ctl->longest = blocks;
-            all += blocks;
+            all += blocks + kUnitCost;
         }
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
@@ -201,7 +204,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
     __syncthreads();
     const int tiles = by_unit ? n_line : min(n_line, (int)gridDim.x);
     blp.total_tiles = tiles;
-    auto on_line = [&](const Unit &u) { return by_unit ? 1 : blocks_of(u); };  // what a unit takes of the line
+    auto on_line = [&](const Unit &u) { return by_unit ? 1 : kUnitCost + blocks_of(u); };  // what a unit takes of the line
     const LmCut cut(n_line, tiles);
     int *const note = p.counters + kLmCounters - kNotes + 4 * blockIdx.x;
     float *const spill = p.parts + (size_t)(p.max_tiles - (int)gridDim.x + (int)blockIdx.x) * Cfg::kSlot;
@@ -269,7 +272,11 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 x.u = lay.unit(s, head * rb_count + rb);
                 x.unit_blocks = blocks_of(x.u);
                 if (by_unit) x.b0 = 0, x.b1 = x.unit_blocks, x.done = ctl->done;
-                else x.b0 = max(x.line0 - x.unit0, 0), x.b1 = min(line1 - x.unit0, x.unit_blocks), x.done = at - x.unit0;
+                else {
+                    const int first = x.unit0 + kUnitCost;  // the place of its first block
+                    x.b0 = max(x.line0 - first, 0), x.b1 = min(line1 - first, x.unit_blocks), x.done = max(at - first, 0);
+                    if (x.b1 <= 0) break;  // (the tile ends before its first block)
+                }
                 x.blocks = min(x.b1, max(0, (x.u.high - x.u.key0 + kTileKeys - 1) / kTileKeys));
                 x.whole = x.b0 == 0 && x.b1 == x.unit_blocks, x.ran = ran;
                 x.two = x.u.rows > 128;
@@ -282,13 +289,13 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 tc_fence_after_sync();
                 if (ctl->stopped) {
                     if (tid == 0) {
-                        note[0] = x.tile + 1, note[1] = by_unit ? ctl->end : x.unit0 + ctl->end - x.line0, note[2] = ctl->end > x.b0;
+                        note[0] = x.tile + 1, note[1] = by_unit ? ctl->end : max(x.unit0 + kUnitCost + ctl->end - x.line0, 0), note[2] = ctl->end > x.b0;
                         atomicCAS(blp.stop_index, -1, blp.kernel_id);
                     }
                     return;
                 }
                 if (!x.whole) {
-                    const int t0 = cut.tile_of(x.unit0), t1 = cut.tile_of(x.unit0 + x.unit_blocks - 1);
+                    const int first = x.unit0 + kUnitCost, t0 = cut.tile_of(first), t1 = cut.tile_of(first + x.unit_blocks - 1);
                     if (tid == 0) {
                         __threadfence();
                         ctl->last = atomicAdd(&p.counters[t0], 1) == t1 - t0;
@@ -766,7 +773,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             }
         }
         const bool to_context = unfinished || !x.whole;
-        float *slot = unfinished ? spill : p.parts + (size_t)(2 * x.tile + (x.unit0 + x.b0 > x.line0 ? 1 : 0)) * Cfg::kSlot;
+        float *slot = unfinished ? spill : p.parts + (size_t)(2 * x.tile + (x.unit0 + kUnitCost + x.b0 > x.line0 ? 1 : 0)) * Cfg::kSlot;
         // (a row without keys is zero; one whose keys all score -infinity is not a number, as the formula says)
         const bool empty = hi <= 0;
         const float inv = empty ? 0.f : unit / l;
@@ -829,7 +836,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         const int row_at = u.row0 + r;
         const long long token = u.first + row_at / group;
         const int q_head = u.head * group + row_at % group;
-        const int slot0 = 2 * t0 + (x.unit0 > cut.begin(t0) ? 1 : 0), parts = t1 - t0 + 1;
+        const int slot0 = 2 * t0 + (x.unit0 + kUnitCost > cut.begin(t0) ? 1 : 0), parts = t1 - t0 + 1;
         auto slot_of = [&](int q) { return p.parts + (size_t)(q == 0 ? slot0 : 2 * (t0 + q)) * Cfg::kSlot; };
         float m = -INFINITY, l = 0.f;
         for (int q = 0; q < parts; ++q) m = fmaxf(m, __ldcg(slot_of(q) + r));
