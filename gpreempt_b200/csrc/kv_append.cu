@@ -391,6 +391,8 @@ static cudaError_t append_launch(const AppendParams &p, int dim, bool half, cons
     const int mode = p.rotated != dim ? TURN_ANY : p.paired ? TURN_PAIRS : TURN_HALVES;
     return append_instance(dim, half, mode, [&](auto one, auto any) {
         int per_sm;
+        // One token a sequence at most: rows are independent, a group of lanes takes each.  (Device time with this kernel and with the
+        // general one, 32 heads of 128 on 8: one sequence 4.4 and 6.1 us, 64 of them 4.9 and 10.8.)
         if (p.batch.most_new == 1) {
             const long long rows = (long long)p.batch.seqs * (2 * p.kv_heads + (p.q ? p.heads : 0));
             const int a_tile = kAppendOneThreads / (dim / 8);

@@ -54,8 +54,8 @@ struct Unit {
     int low, high;                // keys that some row sees: [low, high)
 };
 
-// KEYS: of a block.   All units of a sequence count as many blocks as the longest, so that the place of a block can be
-// computed.
+// How a sequence falls into units of ROWS rows and blocks of KEYS keys.  Where line() is used, all units of a sequence
+// count as many blocks as the longest, so that the place of a block can be computed.
 template <int ROWS, int KEYS>
 struct Layout {
     const AttendParams &p;

@@ -15,8 +15,11 @@
 //
 // What bounds it: 256 x 128 exponentials a block are 2 048 cycles of the special-function unit, the products 2 048
 // of the tensor cores, and shared memory carries 320 KB for them (2 500 cycles).  The halves of the rows are
-// half a block apart, so that one's products run under the other's softmax.  Chunks of 2 048 and 1 161 tokens over contexts of
-// 8 192 and 3 514, 32 heads of 128 on 8: 512 us (557 TFLOP/s), 2 300 with the kernel for few rows.
+// half a block apart, so that one's products run under the other's softmax, and a block takes 3 600 cycles: 2 050 from a
+// half's scores to its factors, 1 450 from those to its next scores.  (Four warpgroups for the scores, two threads a row,
+// took as long for the factors and 300 more to agree on them: 391 us against 362.)  The start and end of a unit take another
+// 25 000.  Chunks of 2 048 and 889 tokens over contexts of 8 192 and 3 474, 32 heads of 128 on 8: 323 us (875 TFLOP/s), 2 300
+// with the kernel for few rows.
 //
 // A tile can last hundreds of microseconds.  The fetching warp reads the preempt word before every block; once it is
 // raised the tile ends behind the blocks under way, sums and statistics go to the context, and the next launch goes on from there.
@@ -44,8 +47,11 @@ constexpr unsigned long long kManyWaitNs = 2000000000ull;
 constexpr float kMostFactors = 32768.f;
 // What the start of a unit takes (queries, the first blocks until their products run, outputs), in blocks: that many places of the
 // line come before its own, so that a tile of many short units has as long as one of a single long unit.
+// (Chunks of 2 048 and 889 tokens: 350 us without, 325 with 6, 323 with 8 and 10, 325 with 14.)
 constexpr int kUnitCost = 8;
-// Blocks of the longest unit up to which units are not cut.
+// Blocks of the longest unit up to which units are not cut.  Uncut and cut, 32 heads of 128 on 8: 8 sequences of 37 tokens over 512
+// keys 21.5 and 24.0 us, 2 of 64 over 764 (6 blocks) 29.6 and 35.9.  With units of 9 to 13 blocks it depends on how they fill
+// the SMs: 8 of 64 over 1 064 37.7 and 41.9, 2 of 64 over 1 564 44.6 and 41.9.
 constexpr int kShortUnit = 8;
 constexpr int kNotes = 1024;  // the last counters of the context: {tile + 1, blocks done, whether sums were left} of a CTA's unfinished tile
 
@@ -59,6 +65,7 @@ struct ManyCfg {
     static constexpr int kSlot = 2 * kTileRows + kTileRows * D;  // floats: maxima, sums, outputs [D / 4][row][4]
 };
 
+// Sequences whose sums have room in what the operands leave of shared memory; sums of more are read from the context.
 constexpr int kFewSeqs = 128;
 
 struct ManyCtl {
@@ -577,7 +584,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             uint4 v[D / 8];
             {
                 const Rows at(base + w * Cfg::kQ, wid, lane);
-                const long long own = token * p.q_ld + (long long)q_head * D;  // (rows past the last have its queries: a condition would make one load wait for another)
+                const long long own = token * p.q_ld + (long long)q_head * D;
+                // (rows past the last have its queries: with a condition, each load waited for the one before)
 #pragma unroll
                 for (int i = 0; i < Rows::kLanes; ++i) {
                     const long long from = __shfl_sync(0xffffffffu, own, at.first + i);
