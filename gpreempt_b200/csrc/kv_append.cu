@@ -397,13 +397,14 @@ static cudaError_t append_launch(const AppendParams &p, int dim, bool half, cons
             const long long rows = (long long)p.batch.seqs * (2 * p.kv_heads + (p.q ? p.heads : 0));
             const int a_tile = kAppendOneThreads / (dim / 8);
             blp.total_tiles = (int)((rows + a_tile - 1) / a_tile);
-            const cudaError_t e = lm_resident((const void *)one, kAppendOneThreads, 0, device, &per_sm);
+            const cudaError_t e = lm_resident((const void *)one, kAppendOneThreads, 0, 0, device, &per_sm);
             if (e != cudaSuccess) return e;
             const int grid = (int)std::min<long long>(blp.total_tiles, (long long)sm_count * per_sm);
             return launch_layer(one, grid, kAppendOneThreads, 0, s, p, blp);
         }
-        const size_t smem = (size_t)page_tokens * dim * 6 + (p.batch.seqs + 1) * sizeof(int);
-        const cudaError_t e = lm_resident((const void *)any, kAppendThreads, smem, device, &per_sm);
+        const size_t smem = (size_t)page_tokens * dim * 6 + lm_prefix_bytes(p.batch.seqs);
+        const size_t most = (size_t)kMostPageTokens * dim * 6 + lm_prefix_bytes(kLmMaxSeqs);
+        const cudaError_t e = lm_resident((const void *)any, kAppendThreads, smem, most, device, &per_sm);
         if (e != cudaSuccess) return e;
         // (pages that new tokens can touch: full ones, and two parts of one a sequence)
         const long long tiles = ((long long)p.batch.tokens / page_tokens + 2ll * std::min(p.batch.seqs, p.batch.tokens)) * p.kv_heads;

@@ -665,9 +665,10 @@ constexpr int kBlocksATile = 16;  // of a preemptible launch: 1024 keys, 256 KiB
 cudaError_t kv_attend_few_launch(AttendParams &p, int dim, bool half, const DeviceInfo &d, const BlpArgs &blp, cudaStream_t s) {
     const int rows = (int)std::min<long long>((long long)p.batch.most_new * (p.heads / p.kv_heads), 1 << 20);
     return attend_instance(dim, rows, half, [&](auto kernel, size_t smem, int tile_rows) {
-        smem += (p.batch.seqs + 1) * sizeof(int);
+        const size_t most = smem + lm_prefix_bytes(kLmMaxSeqs);
+        smem += lm_prefix_bytes(p.batch.seqs);
         int per_sm;
-        const cudaError_t e = lm_resident((const void *)kernel, kAttThreads, smem, d.device, &per_sm);
+        const cudaError_t e = lm_resident((const void *)kernel, kAttThreads, smem, most, d.device, &per_sm);
         if (e != cudaSuccess) return e;
         const size_t slot = (size_t)tile_rows * (dim + 2) * sizeof(float);
         p.max_tiles = (int)std::min<size_t>(kLmCounters, kLmPartsBytes / (2 * slot));

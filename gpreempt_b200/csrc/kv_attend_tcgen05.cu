@@ -905,7 +905,7 @@ cudaError_t kv_attend_many_launch(AttendParams &p, int dim, bool half, const Dev
     auto go = [&](auto kernel, uint32_t fixed, int slot) {
         const size_t smem = 1024 + fixed + sizeof(ManyCtl);
         int per_sm;
-        const cudaError_t e = lm_resident((const void *)kernel, kManyThreads, smem, d.device, &per_sm);
+        const cudaError_t e = lm_resident((const void *)kernel, kManyThreads, smem, smem, d.device, &per_sm);
         if (e != cudaSuccess) return e;
         p.max_tiles = (int)std::min<size_t>(kLmCounters - kNotes, kLmPartsBytes / ((size_t)slot * sizeof(float)));
         // (two parts a tile at most, and an unfinished one)

@@ -63,21 +63,22 @@ int lm_elem(const char *dtype, bool f32_too, int *elem) {
     return GPX_SUCC;
 }
 
-cudaError_t lm_resident(const void *kernel, int threads, size_t smem, int device, int *per_sm) {
+cudaError_t lm_resident(const void *kernel, int threads, size_t smem, size_t most, int device, int *per_sm) {
     struct Known {
         const void *kernel;
-        size_t smem;
+        size_t kib;
         int device, per_sm;
     };
     static thread_local Known table[64] = {};
-    Known &k = table[(reinterpret_cast<uintptr_t>(kernel) >> 4 ^ (uintptr_t)device) % 64];
-    if (k.kernel != kernel || k.smem != smem || k.device != device) {
+    const size_t kib = (smem + 1023) / 1024;
+    Known &k = table[(reinterpret_cast<uintptr_t>(kernel) >> 4 ^ (uintptr_t)device ^ kib) % 64];
+    if (k.kernel != kernel || k.kib != kib || k.device != device) {
         cudaError_t e = cudaSuccess;
-        if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (most > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         int n = 0;
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, kib * 1024);
         if (e != cudaSuccess) return e;
-        k = Known{kernel, smem, device, n > 1 ? n : 1};
+        k = Known{kernel, kib, device, n > 1 ? n : 1};
     }
     *per_sm = k.per_sm;
     return cudaSuccess;

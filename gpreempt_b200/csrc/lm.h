@@ -23,6 +23,7 @@ namespace gpx {
 // what CTAs have in common: sums over the sequences of a batch, parts of results.
 constexpr int kLmCounters = 65536;
 constexpr int kLmMaxSeqs = 4096;
+constexpr int kMostPageTokens = 128;
 constexpr size_t kLmResetBytes = 256 + kLmCounters * sizeof(int);
 constexpr size_t kLmPartsOffset = kLmResetBytes + (kLmMaxSeqs + 64) * sizeof(int);
 constexpr size_t kLmPartsBytes = (size_t)64 << 20;
@@ -65,9 +66,13 @@ enum { LM_F32 = 0, LM_BF16 = 1, LM_F16 = 2 };
 
 #if defined(__CUDACC__)
 
-// CTAs of a kernel an SM holds, asked for once a thread, device and size of shared memory (the question costs more
-// than a small launch).
-cudaError_t lm_resident(const void *kernel, int threads, size_t smem, int device, int *per_sm);
+// CTAs of a kernel that an SM holds with `smem` bytes of dynamic shared memory, of which no launch of it asks for more than
+// `most`.  Asked for once a thread, device and KiB (the question costs more than a small launch).  The limit of a kernel's
+// shared memory belongs to the process: it is only ever set to `most`, so that no thread takes it from under another's launch.
+cudaError_t lm_resident(const void *kernel, int threads, size_t smem, size_t most, int device, int *per_sm);
+// Shared memory for the sums over the sequences of a batch, in steps of a KiB (as an SM deals it out): batches of about
+// the same size are of one size here.
+constexpr size_t lm_prefix_bytes(int seqs) { return ((size_t)(seqs + 1) * sizeof(int) + 1023) / 1024 * 1024; }
 
 __device__ __forceinline__ void lm_fail(int *error, int code, int where) {
     if (atomicCAS(error, 0, code) == 0) error[1] = where;

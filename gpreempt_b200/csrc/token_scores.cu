@@ -609,7 +609,7 @@ extern "C" int gpx_token_scores(const gpx_token_scores_args *args, void *ctx, co
     const bool top = a.top_ids || a.top_logprob;
     int per_sm = 0;
     GPX_CUDA(scores_instance(elem, top, [&](auto kernel) {
-        return lm_resident((const void *)kernel, kScoreThreads, 0, d.device, &per_sm);
+        return lm_resident((const void *)kernel, kScoreThreads, 0, 0, d.device, &per_sm);
     }));
     // Few rows are cut so that two thirds of the warps have a part, of a vector a lane at least.  From half as many rows
     // as warps on they are left whole: a unit costs ~4 us beside its elements, and memory is busy with fewer warps, too
