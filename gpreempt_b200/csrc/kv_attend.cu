@@ -13,7 +13,8 @@
 //
 // The values' scales join the exponents: what multiplies a code is 2^(s_rj + b_j - M_r), b_j = log2 v_scale, with M the running
 // maximum of s + b, so that the largest factor is 1 and none that counts leaves the range of a half, however far apart
-// the scales of pages are; the normaliser adds it times 2^(-b_j).  Factors of fp16 results go through the tensor cores in
+// the scales of pages are; the normaliser adds it times 2^(B - b_j), with B the largest b so far, and is brought to the new B
+// when that grows (a page of zeros has the smallest scale there is: sums that count in a first page's scale vanish behind it).  Factors of fp16 results go through the tensor cores in
 // two halves (22 bits), those of bf16 results in one (11 bits against the result's 8).  Statistics and sums are float.
 //
 // Four warps take sixteen keys each of a block of 64, with a running maximum and output of their own, and are merged
@@ -289,8 +290,9 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 const int pos0 = u.context - u.n + u.row0 / group, pos1 = u.context - u.n + (u.row0 + u.rows - 1) / group;
                 const int all_hi = p.causal ? min(u.context, pos0 + 1) : u.context;
                 const int all_lo = p.window ? pos1 + 1 - p.window : 0;
-                // log2 of value scales: of the first block (the normaliser counts in it), the largest, what `times` belongs to
-                float first_b = 0.f, most_b = -INFINITY, times_b = 0.f, times = 1.f;
+                // log2 of the largest value scale so far, in which the normaliser counts: l is in units of 2^(m - most_b).
+                // times = 2^below, with `below` what a block's scale lies below the largest
+                float most_b = -INFINITY, below = 0.f, times = 1.f;
 
                 for (int b = 0; b < blocks_live; ++b) {
                     wait(&ctl->full[stage], phase);
@@ -338,10 +340,30 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     }
                     // ---- scores: factors, masks where a row's border lies in the block.  A scale 2^40 below the largest counts
                     // as that (or its keys would vanish from the normaliser) and the rest goes into the operand.
-                    if (most_b == -INFINITY) first_b = b_true;
-                    most_b = fmaxf(most_b, b_true);
+                    if (b_true > most_b) {
+                        // (rare, the same for the warp) The sums go to the new unit.  Where that takes a normaliser beyond 2^40, its row's
+                        // reference is raised instead: what then leaves the range of the factors is 2^-64 of the row's weight.
+                        if (most_b != -INFINITY) {
+                            const float d = b_true - most_b;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    float most = l[nt][c];
+                                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
+                                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                                    const float raise = fmaxf(log2f(most) + d - 40.f, 0.f), f = lm_ex2(-raise);
+                                    m[nt][c] += raise;
+                                    l[nt][c] *= lm_ex2(d - raise);
+#pragma unroll
+                                    for (int i = 0; i < MT; ++i) o[nt][i][c] *= f, o[nt][i][c + 2] *= f;
+                                }
+                        }
+                        most_b = b_true;
+                    }
                     const float b_used = fmaxf(b_true, most_b - 40.f);
-                    if (b_used != times_b || b == 0) times_b = b_used, times = lm_ex2(first_b - b_used);
+                    if (most_b - b_used != below) below = most_b - b_used, times = lm_ex2(below);
                     const int block_key = u.key0 + (block0 + b) * kAttKeys;
                     const bool border = block_key + kAttKeys > all_hi || block_key < all_lo;
                     uint32_t seen = ~0u;  // bit 4 nt + c
@@ -469,12 +491,12 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     }
                 }
 
-                // ---- the four warps' results as one: warps 2 and 3 into 0 and 1, 1 into 0.  l counts in 2^(m - first_b).
-                const float unit_scale = lm_ex2(first_b);
+                // ---- the four warps' results as one: warps 2 and 3 into 0 and 1, 1 into 0.  l counts in 2^(m - most_b).
+                const float unit = blocks_live ? most_b : 0.f, unit_scale = lm_ex2(unit);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) m[nt][c] -= first_b;
+                    for (int c = 0; c < 2; ++c) m[nt][c] -= unit;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

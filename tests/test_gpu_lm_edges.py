@@ -5,7 +5,8 @@ import threading
 import numpy as np
 import pytest
 
-from test_gpu_lm import Bed, to_bits
+from oracle import lm
+from test_gpu_lm import BITS, Bed, from_bits, run_attention, to_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -16,6 +17,19 @@ def ctx(gpx):
     yield c
     assert c.status() == (0, 0)
     c.free()
+
+
+def check(got, ref, weight, dtype, p_bits, score_err, keys, vmax):
+    """What the formats allow: the result is rounded once; a factor of a product is rounded to `p_bits` bits and loses at most
+    2^-31 of the largest; a score is off by `score_err`.  No absolute term: a result may be small as a whole."""
+    assert np.array_equal(np.isnan(got), np.isnan(ref))
+    allowed = 1.01 * 2.0 ** -BITS[dtype] * np.abs(ref) + (2.0 ** -p_bits + 2 * score_err) * weight + 2.0 ** -31 * keys * vmax
+    worst = np.max(np.abs(got.astype(np.float64) - ref) / allowed)
+    assert worst <= 1, worst
+
+
+def values_largest(bed):
+    return float(np.max(np.abs(lm.decode(bed.v)).max((2, 3)) * bed.vs))
 
 
 # ---- threads ----------------------------------------------------------------------------------------
@@ -68,3 +82,43 @@ def test_threads_with_batches_of_their_own(gpx):
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+# ---- scales and scores far apart ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [1, 3, 8, 20])
+@pytest.mark.parametrize("power", [-8, 1, 3, 60])
+def test_first_pages_of_zeros(gpx, ctx, new, power):
+    """A page of zeros, as append stores it, before pages of any scale, with many blocks a tile."""
+    seqs, c, heads, kv, dim, page, dtype = 48, 1200, 32, 8, 64, 16, "bfloat16"
+    bed = Bed(gpx, [new] * seqs, [c] * seqs, heads, kv, dim, page, seed=new)
+    bed.vs[:] = 2.0 ** power
+    bed.v[bed.table[:, 0]], bed.vs[bed.table[:, 0]] = 0, 2.0 ** -126
+    bed.upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), dtype), dtype)
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads)
+    some = 4 * new
+    ref, ref_lse, weight = lm.attend(q[:some], bed.k, bed.v, bed.ks, bed.vs, bed.table, bed.context[:4], bed.first[:5])
+    check(got[:some], ref, weight, dtype, 11, 2.0 ** -14, c, values_largest(bed))
+    assert np.all(np.abs(lse[:some] - ref_lse) <= 2.0 ** -14)
+    bed.free()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_page_of_zeros_does_not_hide_what_other_warps_see(gpx, ctx, dim):
+    """One key 2^10 ahead of 1 200 others that weigh as much together, in the sixteen keys of a block whose first page is zeros."""
+    seqs, c, heads, kv, page, dtype = 48, 1200, 16, 8, 16, "bfloat16"
+    bed = Bed(gpx, [1] * seqs, [c] * seqs, heads, kv, dim, page, seed=dim)
+    bed.vs[:] = 2.0 ** -8
+    bed.v[bed.table[:, 0]], bed.vs[bed.table[:, 0]] = 0, 2.0 ** -126
+    bed.k[..., 0], bed.ks[:] = 0, 1.0
+    bed.k[bed.table[:, 12], :, 2, 0] = 0x7E  # 448, key 194 of each
+    bed.upload()
+    q = np.zeros((bed.tokens, heads, dim), np.float32)
+    q[..., 0] = 1
+    scale = float(np.float32(10 * np.log(2) / 448))
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads, scale=scale)
+    ref, ref_lse, weight = lm.attend(q[:4], bed.k, bed.v, bed.ks, bed.vs, bed.table, bed.context[:4], bed.first[:5], scale)
+    check(got[:4], ref, weight, dtype, 11, 2.0 ** -17, c, values_largest(bed))
+    assert np.all(np.abs(lse[:4] - ref_lse) <= 2.0 ** -17)
+    bed.free()
