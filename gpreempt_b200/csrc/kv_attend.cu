@@ -11,9 +11,9 @@
 // of two that brings their row's largest to 1; the scores' factors (that power, the page's scale, scale, log2 e) are
 // applied to the sums.
 //
-// The values' scales join the exponents: what multiplies a code is 2^(s_rj + b_j - M_r), b_j = log2 v_scale, with M the running
-// maximum of s + b, so that the largest factor is 1 and none that counts leaves the range of a half, however far apart
-// the scales of pages are; the normaliser adds it times 2^(B - b_j), with B the largest b so far, and is brought to the new B
+// The values' scales join the exponents: what multiplies a code is 2^14 2^(s_rj + b_j - M_r), b_j = log2 v_scale, with M the running
+// maximum of s + b, so that none that counts leaves the range of a half, however far apart the scales of pages are, nor does the sum of
+// thousands of keys that weigh 2^-26 each beside one that weighs 1 (a half ends at 2^-25 below and 2^16 above); the normaliser adds it times 2^(B - b_j), with B the largest b so far, and is brought to the new B
 // when that grows (a page of zeros has the smallest scale there is: sums that count in a first page's scale vanish behind it).  Factors of fp16 results go through the tensor cores in
 // two halves (22 bits), those of bf16 results in one (11 bits against the result's 8).  Statistics and sums are float.
 //
@@ -39,6 +39,8 @@ using namespace sm100;
 
 constexpr int kAttWarps = 4, kAttConsumers = 32 * kAttWarps, kAttThreads = kAttConsumers + 32;
 constexpr int kAttKeys = 64;
+constexpr float kLift = 16384.f;  // of the factors as operands
+constexpr int kSumBlocks = 16;
 constexpr unsigned long long kAttWaitNs = 2000000000ull;
 
 template <int D, int NT>
@@ -266,7 +268,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     for (int k = 0; k < KS; ++k) qr[k] = q_frag[k * 32 + lane];
                 }
                 // this lane's columns: rows 8 nt + 2 t and the next
-                float mult[NT][2], m[NT][2], l[NT][2];
+                float mult[NT][2], m[NT][2], l[NT][2], before[NT][2];  // (l: of the last kSumBlocks blocks, before: of those ahead)
                 int lo[NT][2], hi[NT][2];
                 float o[NT][MT][4];
 #pragma unroll
@@ -275,7 +277,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     for (int c = 0; c < 2; ++c) {
                         const int r = min(8 * nt + 2 * t + c, u.rows - 1);
                         mult[nt][c] = ctl->row_factor[8 * nt + 2 * t + c] * p.scale * 1.4426950408889634f;
-                        m[nt][c] = -INFINITY, l[nt][c] = 0.f;
+                        m[nt][c] = -INFINITY, l[nt][c] = before[nt][c] = 0.f;
                         const int pos = u.context - u.n + (u.row0 + r) / group;
                         hi[nt][c] = p.causal ? min(u.context, pos + 1) : u.context;
                         lo[nt][c] = p.window ? pos + 1 - p.window : 0;
@@ -341,21 +343,22 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     // ---- scores: factors, masks where a row's border lies in the block.  A scale 2^40 below the largest counts
                     // as that (or its keys would vanish from the normaliser) and the rest goes into the operand.
                     if (b_true > most_b) {
-                        // (rare, the same for the warp) The sums go to the new unit.  Where that takes a normaliser beyond 2^40, its row's
-                        // reference is raised instead: what then leaves the range of the factors is 2^-64 of the row's weight.
+                        // (rare, the same for the warp) The sums go to the new unit.  Where that takes a normaliser beyond 2^64, its row's
+                        // reference is raised instead: what then leaves the range of the factors is 2^-100 of the row's weight.
                         if (most_b != -INFINITY) {
                             const float d = b_true - most_b;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    float most = l[nt][c];
+                                    float most = l[nt][c] + before[nt][c];
                                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
                                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                                    const float raise = fmaxf(log2f(most) + d - 40.f, 0.f), f = lm_ex2(-raise);
+                                    const float raise = fmaxf(log2f(most) + d - 64.f, 0.f), f = lm_ex2(-raise);
                                     m[nt][c] += raise;
-                                    l[nt][c] *= lm_ex2(d - raise);
+                                    const float up = lm_ex2(d - raise);
+                                    l[nt][c] *= up, before[nt][c] *= up;
 #pragma unroll
                                     for (int i = 0; i < MT; ++i) o[nt][i][c] *= f, o[nt][i][c + 2] *= f;
                                 }
@@ -398,12 +401,19 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                                 const float now = fmaxf(m[nt][c], x);
                                 const float f = now == -INFINITY ? 1.f : lm_ex2(m[nt][c] - now);
                                 m[nt][c] = now;
-                                l[nt][c] *= f;
+                                l[nt][c] *= f, before[nt][c] *= f;
 #pragma unroll
                                 for (int i = 0; i < MT; ++i) o[nt][i][c] *= f, o[nt][i][c + 2] *= f;
                             }
                     }
-                    const float p_factor = b_used != b_true ? lm_ex2(b_true - b_used) : 1.f;
+                    if (b % kSumBlocks == 0) {
+                        // (thousands of blocks that are small beside one of the first would vanish in one sum)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) before[nt][c] += l[nt][c], l[nt][c] = 0.f;
+                    }
+                    const float p_factor = b_used != b_true ? kLift * lm_ex2(b_true - b_used) : kLift;
                     uint32_t pb[NT][2], pl[kTwo ? NT : 1][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -492,7 +502,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 }
 
                 // ---- the four warps' results as one: warps 2 and 3 into 0 and 1, 1 into 0.  l counts in 2^(m - most_b).
-                const float unit = blocks_live ? most_b : 0.f, unit_scale = lm_ex2(unit);
+                const float unit = blocks_live ? most_b : 0.f, unit_scale = lm_ex2(unit);  // (and o 2^14 times as much)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -501,6 +511,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
+                        l[nt][c] += before[nt][c];
 #pragma unroll
                         for (int d = 4; d <= 16; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
                         if (g == 0) {
@@ -523,9 +534,9 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 #pragma unroll
                         for (int w = 0; w < kAttWarps; ++w) all += ctl->ml[w][r][1] * lm_ex2(ctl->ml[w][r][0] - ref);
                         most[nt][c] = mm, sum[nt][c] = all;
-                        const float f = lm_ex2(m[nt][c] - ref) * unit_scale;
+                        const float f = lm_ex2(m[nt][c] - ref) * (1.f / kLift);
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) o[nt][i][c] *= f, o[nt][i][c + 2] *= f;
+                        for (int i = 0; i < MT; ++i) o[nt][i][c] = o[nt][i][c] * f * unit_scale, o[nt][i][c + 2] = o[nt][i][c + 2] * f * unit_scale;
                     }
 #pragma unroll
                 for (int round = 2; round >= 1; round >>= 1) {

@@ -41,10 +41,10 @@ constexpr int kManyRegs = 168, kFewRegs = 88;
 constexpr int kTileRows = 256, kTileKeys = 128;
 constexpr int kRawStages = 2, kKeyBuffers = 2, kValueBuffers = 2;  // (a stage of the ring holds a block's keys or its values)
 constexpr unsigned long long kManyWaitNs = 2000000000ull;
-// A row's exponents refer to its maximum in the first block it sees until their factors sum to more than this in a block, which a
-// half holds; then the maximum is taken anew and the sums are rescaled.  (Asking for the maximum of every block goes
+// A row's exponents refer to kLift below its maximum in the first block it sees (so that thousands of keys that weigh 2^-26 each beside one
+// of that block count: a half ends at 2^-25) until their factors sum to more than this in a block, which a half holds; then the maximum is taken anew and the sums are rescaled.  (Asking for the maximum of every block goes
 // through its scores twice, and a new one among 32 rows, which are rescaled together, comes in most blocks.)
-constexpr float kMostFactors = 32768.f;
+constexpr float kMostFactors = 60000.f, kLift = 6.f;
 // What the start of a unit takes (queries, the first blocks until their products run, outputs), in blocks: that many places of the
 // line come before its own, so that a tile of many short units has as long as one of a single long unit.
 // (Chunks of 2 048 and 889 tokens: 350 us without, 325 with 6, 323 with 8 and 10, 325 with 14.)
@@ -82,6 +82,9 @@ struct ManyCtl {
     int saw_nan, last, longest, abort_flag;
     int prefix[kFewSeqs];
 };
+
+// Of exponents of 2^20 and more the largest itself: it has no bits for the difference.
+__device__ __forceinline__ float reference_of(float largest) { return fabsf(largest) < 1048576.f ? largest - kLift : largest; }
 
 // The largest of three (one instruction on this architecture).
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -719,11 +722,11 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     }
                 }
             };
-            // The maximum of the first block that a row sees is its first reference.  Later ones are not asked for theirs: where
-            // the factors of a row sum to less than 2^15 none has left the range of a half.
+            // The maximum of the first block that a row sees gives its first reference.  Later ones are not asked for theirs: where
+            // the factors of a row sum to kMostFactors at most none has left the range of a half.
             if (__any_sync(0xffffffffu, m == -INFINITY)) {
                 const float most = largest();
-                if (m == -INFINITY) m = most;
+                if (m == -INFINITY) m = reference_of(most);
             }
             // (Exponents of 2^20 and more are rounded first throughout: one sum with the reference would leave the largest off 0 by
             // up to 2^-24 of itself, which can be more than the range of a half.  So it is where the pass is repeated.)
@@ -734,7 +737,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 // (once is enough, unless a page's scale is not positive, which is no reason to go on without end)
                 if (pass || !__any_sync(0xffffffffu, plain > kMostFactors)) break;
                 // (the scores' arrival means that the products before them are complete)
-                const float now = fmaxf(m, largest()), f = now == -INFINITY ? 1.f : lm_ex2(m - now);
+                const float now = fmaxf(m, reference_of(largest())), f = now == -INFINITY ? 1.f : lm_ex2(m - now);
 #pragma unroll 1
                 for (int c = 0; j > x.b0 && c < D; c += 32) {
                     uint32_t o[32];

@@ -122,3 +122,26 @@ def test_a_page_of_zeros_does_not_hide_what_other_warps_see(gpx, ctx, dim):
     check(got[:4], ref, weight, dtype, 11, 2.0 ** -17, c, values_largest(bed))
     assert np.all(np.abs(lse[:4] - ref_lse) <= 2.0 ** -17)
     bed.free()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("new,seqs", [(1, 444), (5, 444), (40, 148)])
+def test_a_first_key_that_holds_most_of_the_weight(gpx, ctx, dtype, new, seqs):
+    """Sixty thousand keys of 2^-25.6 each behind it, with values 448 times its own: they are a third of the result."""
+    c, heads, kv, dim, page = 60000, 1, 1, 64, 128
+    bed = Bed(gpx, [new], [c], heads, kv, dim, page, seed=1)
+    bed.k[:], bed.v[:], bed.ks[:], bed.vs[:] = 0, 0x7E, 1.0, 1.0
+    bed.k[bed.table[0, 0], 0, 0, 0], bed.v[bed.table[0, 0], 0, 0] = 0x7E, 0x38  # 448, and 1
+    # (all sequences have the same pages)
+    bed.table = np.repeat(bed.table, seqs, 0)
+    bed.new, bed.context, bed.tokens = [new] * seqs, np.full(seqs, c, np.int32), new * seqs
+    bed.first = (np.arange(seqs + 1) * new).astype(np.int32)
+    bed.upload()
+    q = np.zeros((bed.tokens, heads, dim), np.float32)
+    q[..., 0] = 1
+    scale = float(np.float32(25.6 * np.log(2) / 448))
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads, causal=False, scale=scale)
+    ref, ref_lse, weight = lm.attend(q[:1], bed.k, bed.v, bed.ks, bed.vs, bed.table[:1], [c], [0, 1], scale, causal=False)
+    check(got, np.broadcast_to(ref, got.shape), np.broadcast_to(weight, got.shape), dtype, 11, 2.0 ** -17, c, 448.0)
+    assert np.all(np.abs(lse - ref_lse[0, 0]) <= 2.0 ** -17)
+    bed.free()
