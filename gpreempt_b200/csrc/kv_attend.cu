@@ -357,7 +357,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                                     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
                                     const float raise = fmaxf(log2f(most) + d - 64.f, 0.f), f = lm_ex2(-raise);
                                     m[nt][c] += raise;
-                                    const float up = lm_ex2(d - raise);
+                                    const float up = lm_ex2(fminf(d - raise, 126.f));  // (a row without keys so far has no sum, and its d no bound)
                                     l[nt][c] *= up, before[nt][c] *= up;
 #pragma unroll
                                     for (int i = 0; i < MT; ++i) o[nt][i][c] *= f, o[nt][i][c + 2] *= f;

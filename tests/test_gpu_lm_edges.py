@@ -104,6 +104,26 @@ def test_first_pages_of_zeros(gpx, ctx, new, power):
     bed.free()
 
 
+@pytest.mark.parametrize("new", [4, 8])
+@pytest.mark.parametrize("power", [-8, 3, 100])
+def test_rows_that_do_not_see_a_page_of_zeros(gpx, ctx, new, power):
+    """A page of zeros at the lower end of a window: the later of the new tokens see none of it, and have no sum when the scale grows."""
+    seqs, c, heads, kv, dim, page, dtype, window = 40, 1000, 32, 8, 64, 16, "bfloat16", 900
+    bed = Bed(gpx, [new] * seqs, [c + i for i in range(seqs)], heads, kv, dim, page, seed=new)
+    bed.vs[:] = 2.0 ** power
+    for s in range(seqs):
+        first = bed.table[s, (c + s - new + 1 - window) // page]
+        bed.v[first], bed.vs[first] = 0, 2.0 ** -126
+    bed.upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), dtype), dtype)
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads, window=window)
+    some = 16 * new
+    ref, ref_lse, weight = lm.attend(q[:some], bed.k, bed.v, bed.ks, bed.vs, bed.table, bed.context[:16], bed.first[:17], window=window)
+    check(got[:some], ref, weight, dtype, 11, 2.0 ** -14, c, values_largest(bed))
+    assert np.all(np.abs(lse[:some] - ref_lse) <= 2.0 ** -14)
+    bed.free()
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_a_page_of_zeros_does_not_hide_what_other_warps_see(gpx, ctx, dim):
     """One key 2^10 ahead of 1 200 others that weigh as much together, in the sixteen keys of a block whose first page is zeros."""
