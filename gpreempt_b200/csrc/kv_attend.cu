@@ -173,8 +173,9 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     const int mine = lane / pieces, sub = lane - mine * pieces;
                     const int key = u.key0 + (block0 + b0 + mine) * kAttKeys + sub * per_page;
                     int row = -1;
-                    float ks = 1.f, vs = 1.f;
-                    if (b0 + mine < blocks_live && key < u.high) {
+                    float ks = 1.f, vs = 0.f;
+                    // (what ends below the keys that are seen may be anybody's by now: neither fetched nor asked for its scale)
+                    if (b0 + mine < blocks_live && key < u.high && key + per_page > u.low) {
                         const int page = p.batch.table[(size_t)u.s * p.batch.table_ld + (key >> p.page_shift)];
                         if ((unsigned)page < (unsigned)p.pages) {
                             const long long block = (long long)page * p.kv_heads + u.head;

@@ -352,7 +352,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             const int key = x.key(j + mine) + sub * per_page;
             int row = -1;
             float ks = 1.f, vs = 1.f;
-            if (j + mine < x.blocks && key < u.high) {
+            // (what ends below the keys that are seen may be anybody's by now)
+            if (j + mine < x.blocks && key < u.high && key + per_page > u.low) {
                 const int page = p.batch.table[(size_t)u.s * p.batch.table_ld + (key >> p.page_shift)];
                 if ((unsigned)page < (unsigned)p.pages) {
                     const long long block = (long long)page * p.kv_heads + u.head;
@@ -473,7 +474,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         const int r = tid - 256;
         // the largest scale of the values of the piece
         float most = 0.f;
-        for (int i = (x.key(x.b0) >> p.page_shift) + r; (i << p.page_shift) < min(u.high, x.key(x.b1)); i += 128) {
+        for (int i = (max(x.key(x.b0), u.low) >> p.page_shift) + r; (i << p.page_shift) < min(u.high, x.key(x.b1)); i += 128) {
             const int page = p.batch.table[(size_t)u.s * p.batch.table_ld + i];
             if ((unsigned)page < (unsigned)p.pages) most = fmaxf(most, p.v_scale[(long long)page * p.kv_heads + u.head]);
         }

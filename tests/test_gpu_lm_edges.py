@@ -165,3 +165,35 @@ def test_a_first_key_that_holds_most_of_the_weight(gpx, ctx, dtype, new, seqs):
     check(got, np.broadcast_to(ref, got.shape), np.broadcast_to(weight, got.shape), dtype, 11, 2.0 ** -17, c, 448.0)
     assert np.all(np.abs(lse - ref_lse[0, 0]) <= 2.0 ** -17)
     bed.free()
+
+
+# ---- pages that nothing can see -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["returned", "of others", "small values"])
+@pytest.mark.parametrize("new,context,window,page", [([1, 1], [777, 300], 50, 16), ([4, 1], [900, 64], 37, 32), ([30, 8], [700, 129], 20, 16),
+                                                     ([80, 100], [815, 333], 100, 32), ([300, 40], [1300, 1000], 33, 16), ([1] * 100, [1000 + i for i in range(100)], 300, 16)])
+def test_pages_below_a_window_have_no_influence(gpx, ctx, kind, new, context, window, page):
+    """Pages that no row sees any more: taken out of the table, or somebody else's by now; and the other values as small as they go."""
+    heads, kv, dim, dtype = 4, 2, 128, "bfloat16"
+    bed = Bed(gpx, new, context, heads, kv, dim, page, seed=window)
+    if kind == "small values":
+        bed.vs = np.ldexp(bed.vs, -80)
+    want = [a.copy() for a in (bed.k, bed.v, bed.ks, bed.vs, bed.table)]
+    for s, (n, c) in enumerate(zip(new, context)):
+        dead = max(0, c - n + 1 - window) // page
+        if kind == "returned":
+            bed.table[s, :dead] = -1
+        else:
+            bed.v[bed.table[s, :dead]], bed.k[bed.table[s, :dead]] = 0x7F, 0x7F
+            bed.vs[bed.table[s, :dead]], bed.ks[bed.table[s, :dead]] = 2.0 ** 100, 2.0 ** 90
+    bed.upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), dtype), dtype)
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads, window=window)
+    status = ctx.status()
+    ctx.reset()
+    assert status == (0, 0)
+    ref, ref_lse, weight = lm.attend(q, *want, bed.context, bed.first, None, True, window)
+    bed.v, bed.vs = want[1], want[3]
+    check(got, ref, weight, dtype, 11, 2.0 ** -13, max(context), values_largest(bed))
+    assert np.all(np.abs(lse - ref_lse) <= 2.0 ** -13)
+    bed.free()
