@@ -660,11 +660,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
             const float4 *of = reinterpret_cast<const float4 *>(ctl->scales[j & 3]);  // (by groups of sixteen keys)
             const bool masks = x.border(j);
             const int high = hi - x.key(j), low = lo - x.key(j);
-            auto hide = [&](int c, uint32_t(&v)[32]) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (32 * c + i >= high || 32 * c + i < low) v[i] = 0xff800000u;
-            };
+            auto hides = [&](int i) { return i >= high || i < low; };
             // the largest exponent of the row in this block
             auto largest = [&]() {
                 float most = -INFINITY;
@@ -673,10 +669,15 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                     uint32_t v[32];
                     tmem_ld_32x32(t_s + 32 * c, v);
                     tmem_ld_wait();
-                    if (masks) hide(c, v);
+                    if (masks) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (hides(32 * c + i)) v[i] = 0xff800000u;
+                    }
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const float4 g = of[2 * c + q];
+                        // (of keys that are all hidden -infinity, or not a number, which is no maximum either)
                         float e = __uint_as_float(v[16 * q]);
 #pragma unroll
                         for (int i = 1; i < 16; ++i) e = fmaxf(e, __uint_as_float(v[16 * q + i]));
@@ -704,7 +705,6 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                         tmem_ld_32x32(t_s + 32 * (c + 1), both[(c + 1) & 1]);
                         next[0] = of[2 * c + 2], next[1] = of[2 * c + 3];
                     }
-                    if (decltype(careful)::value) hide(c, v);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const float less = decltype(careful)::value ? g[q].z : g[q].z - ref;
@@ -713,7 +713,8 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 #pragma unroll
                         for (int i = 8 * q; i < 8 * q + 8; ++i) {
                             float2 y = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by, plus);
-                            if (decltype(careful)::value) y.x -= ref, y.y -= ref;
+                            // (hidden behind the factor, which may be as small as zero: that times -infinity is not a number)
+                            if (decltype(careful)::value) y.x = hides(32 * c + 2 * i) ? -INFINITY : y.x - ref, y.y = hides(32 * c + 2 * i + 1) ? -INFINITY : y.y - ref;
                             const float2 e = make_float2(lm_ex2(y.x), lm_ex2(y.y));
                             part[i & 1] = add2(part[i & 1], e);
                             h[16 * c + i] = pack_halves(e.x, e.y);

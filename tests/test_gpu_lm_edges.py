@@ -197,3 +197,21 @@ def test_pages_below_a_window_have_no_influence(gpx, ctx, kind, new, context, wi
     check(got, ref, weight, dtype, 11, 2.0 ** -13, max(context), values_largest(bed))
     assert np.all(np.abs(lse - ref_lse) <= 2.0 ** -13)
     bed.free()
+
+
+# ---- the ends of the types ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [1, 8, 40])
+@pytest.mark.parametrize("power", [-120, -24, -21])
+def test_tiny_queries_over_keys_of_zero(gpx, ctx, new, power):
+    """Scores are zero: a row's result is the mean of what it sees, hidden keys or not."""
+    c, heads, kv, dim, page, dtype = 100 + new, 4, 2, 64, 64, "bfloat16"
+    bed = Bed(gpx, [new], [c], heads, kv, dim, page, seed=new)
+    bed.k[:], bed.ks[:] = 0, 2.0 ** -126
+    bed.upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((new, heads, dim)) * 2.0 ** power, dtype), dtype)
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads)
+    ref, ref_lse, weight = lm.attend(q, bed.k, bed.v, bed.ks, bed.vs, bed.table, [c], bed.first)
+    check(got, ref, weight, dtype, 11, 2.0 ** -19, c, values_largest(bed))
+    assert np.all(np.abs(lse - ref_lse) <= 2.0 ** -19)
+    bed.free()
