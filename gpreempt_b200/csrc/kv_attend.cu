@@ -281,7 +281,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                         m[nt][c] = -INFINITY, l[nt][c] = before[nt][c] = 0.f;
                         const int pos = u.context - u.n + (u.row0 + r) / group;
                         hi[nt][c] = p.causal ? min(u.context, pos + 1) : u.context;
-                        lo[nt][c] = p.window ? pos + 1 - p.window : 0;
+                        lo[nt][c] = first_seen(p, pos);
                     }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -292,7 +292,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 // keys that every row sees: [all_lo, all_hi)
                 const int pos0 = u.context - u.n + u.row0 / group, pos1 = u.context - u.n + (u.row0 + u.rows - 1) / group;
                 const int all_hi = p.causal ? min(u.context, pos0 + 1) : u.context;
-                const int all_lo = p.window ? pos1 + 1 - p.window : 0;
+                const int all_lo = first_seen(p, pos1);
                 // log2 of the largest value scale so far, in which the normaliser counts: l is in units of 2^(m - most_b).
                 // times = 2^below, with `below` what a block's scale lies below the largest
                 float most_b = -INFINITY, below = 0.f, times = 1.f;

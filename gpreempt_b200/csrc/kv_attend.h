@@ -46,6 +46,11 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
 // 0xff in every byte that is e4m3's NaN (all bits but the sign)
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
+// The first key that a row at a position sees (which is negative where there are more new tokens than keys).
+__device__ __forceinline__ int first_seen(const AttendParams &p, int position) {
+    return p.window && position >= p.window ? position - p.window + 1 : 0;
+}
+
 // A unit's place on the line of blocks, and what it covers.
 struct Unit {
     int s, head, row0, rows;      // sequence, head of keys, first of its rows and how many
@@ -83,7 +88,7 @@ struct Layout {
         u.low = 0, u.high = u.context;
         if (p.causal) {
             u.high = max(0, u.context - u.n + (u.row0 + u.rows - 1) / group + 1);
-            if (p.window) u.low = max(0, u.context - u.n + u.row0 / group - p.window + 1);
+            u.low = first_seen(p, u.context - u.n + u.row0 / group);
         }
         u.low = min(u.low, u.high);
         u.key0 = u.low & ~(KEYS - 1);

@@ -292,7 +292,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                 x.two = x.u.rows > 128;
                 const int pos0 = x.u.context - x.u.n + x.u.row0 / group, pos1 = x.u.context - x.u.n + (x.u.row0 + x.u.rows - 1) / group;
                 x.all_hi = p.causal ? min(x.u.context, pos0 + 1) : x.u.context;
-                x.all_lo = p.window ? pos1 + 1 - p.window : 0;
+                x.all_lo = first_seen(p, pos1);
                 role(x);
                 tc_fence_before_sync();
                 __syncthreads();
@@ -626,7 +626,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
         }
         const float mult = factor * p.scale * 1.4426950408889634f;
         const int pos = u.context - u.n + row_at / group;
-        const int hi = p.causal ? min(u.context, pos + 1) : u.context, lo = p.window ? pos + 1 - p.window : 0;
+        const int hi = p.causal ? min(u.context, pos + 1) : u.context, lo = first_seen(p, pos);
         float m = -INFINITY, l = 0.f;
         if (x.goes_on) {
             // an interrupted piece goes on

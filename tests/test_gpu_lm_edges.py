@@ -199,6 +199,23 @@ def test_pages_below_a_window_have_no_influence(gpx, ctx, kind, new, context, wi
     bed.free()
 
 
+@pytest.mark.parametrize("new,context", [(200, 150), (20, 13), (200, 190), (300, 40)])
+def test_the_largest_window_is_no_window(gpx, ctx, new, context):
+    """More new tokens than keys: the first rows' positions are negative."""
+    heads, kv, dim, page, dtype = 4, 2, 64, 16, "bfloat16"
+    bed = Bed(gpx, [new], [context], heads, kv, dim, page, seed=new).upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((new, heads, dim)), dtype), dtype)
+    want = run_attention(gpx, ctx, bed, q, dtype, heads)
+    got = run_attention(gpx, ctx, bed, q, dtype, heads, window=2 ** 31 - 1)
+    ref, _, weight = lm.attend(q, bed.k, bed.v, bed.ks, bed.vs, bed.table, [context], bed.first)
+    for out, lse in (want, got):
+        assert np.array_equal(np.isneginf(lse), np.isneginf(want[1]))
+        seen = np.abs(ref).sum(-1) > 0
+        assert np.all(out[~seen] == 0)
+        check(out[seen], ref[seen], weight[seen], dtype, 11, 2.0 ** -13, context, values_largest(bed))
+    bed.free()
+
+
 # ---- the ends of the types ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("new", [1, 8, 40])
