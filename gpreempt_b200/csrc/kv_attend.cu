@@ -246,9 +246,7 @@ kv_attend_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                         }
                         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
                         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                        // the power of two below the largest, where it and its reciprocal are normal numbers
-                        const uint32_t e = most >> 23;
-                        if (e > 0 && e < 253) factor = __uint_as_float(e << 23);
+                        factor = query_factor(most);
                         const float inv = 1.0f / factor;
 #pragma unroll
                         for (int k = 0; k < KS; ++k) {

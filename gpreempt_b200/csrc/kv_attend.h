@@ -43,6 +43,9 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+// The power of two below a row's largest query (bits of its magnitude), which brings the row's queries into the range of halves; at
+// least 2^-126 and at most 2^125, so that it and its reciprocal are normal numbers (halves have room for what is left of larger ones).
+__device__ __forceinline__ float query_factor(uint32_t most) { return __uint_as_float(min(max(most >> 23, 1u), 252u) << 23); }
 // 0xff in every byte that is e4m3's NaN (all bits but the sign)
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 

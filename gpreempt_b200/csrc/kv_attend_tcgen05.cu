@@ -612,8 +612,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) most = max(most, max(e[i] << 16 & 0x7fffffffu, e[i] & 0x7fff0000u));
                 }
-                const uint32_t e = most >> 23;
-                if (e > 0 && e < 253) factor = __uint_as_float(e << 23);
+                factor = query_factor(most);
                 inv = 1.0f / factor;
             }
 #pragma unroll

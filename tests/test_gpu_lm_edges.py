@@ -232,3 +232,20 @@ def test_tiny_queries_over_keys_of_zero(gpx, ctx, new, power):
     check(got, ref, weight, dtype, 11, 2.0 ** -19, c, values_largest(bed))
     assert np.all(np.abs(lse - ref_lse) <= 2.0 ** -19)
     bed.free()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("power", [-127, 125, 126, 127])
+def test_queries_at_the_ends_of_their_type(gpx, ctx, new, power):
+    """Rows whose largest element is of either end, with keys' scales that bring the scores back to a few units."""
+    c, heads, kv, dim, page, dtype = 100 + new, 4, 2, 128, 64, "bfloat16"
+    bed = Bed(gpx, [new], [c], heads, kv, dim, page, seed=new)
+    bed.ks[:] = 2.0 ** (-10 - power if power > 0 else 118)
+    bed.upload()
+    x = np.clip(bed.rng.standard_normal((new, heads, dim)), -1.9, 1.9).astype(np.float64)
+    q = from_bits(to_bits((x * 2.0 ** power).astype(np.float32), dtype), dtype)
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads)
+    ref, ref_lse, weight = lm.attend(q, bed.k, bed.v, bed.ks, bed.vs, bed.table, [c], bed.first)
+    check(got, ref, weight, dtype, 11, 2.0 ** -13, c, values_largest(bed))
+    assert np.all(np.abs(lse - ref_lse) <= 2.0 ** -13)
+    bed.free()
