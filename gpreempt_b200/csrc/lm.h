@@ -94,21 +94,21 @@ __device__ __forceinline__ LmSpan lm_span(const LmBatch &b, int s, int page_toke
     return {f, e - f, c};
 }
 
-// prefix[s] = sum of count(0 .. s-1), prefix[seqs] = the total, for all threads of the CTA together.  More than
-// 31 bits of them are reported, and nothing is to be done.
+// prefix[s] = sum of count(0 .. s-1), prefix[seqs] = the total, for all threads of the CTA together.  A total of
+// 2^31 - 1 and more is reported, and nothing is to be done; a count of 2^31 - 1 may stand for one beyond.
 template <typename F>
 __device__ __forceinline__ int lm_prefix(int *prefix, int seqs, int *error, F &&count) {
-    __shared__ int s_sums[32];
+    __shared__ unsigned s_sums[32];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
     long long before_all = 0;
     for (int s0 = 0; s0 < seqs; s0 += blockDim.x) {
         const int s = s0 + threadIdx.x;
         const int own = s < seqs ? count(s) : 0;
-        int sum = own;
+        unsigned sum = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += up;
+            const unsigned up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum = min(sum + up, 0x7fffffffu);
         }
         if (s0 > 0) __syncthreads();  // the sums of the round before have been read
         if (lane == 31) s_sums[wid] = sum;
@@ -120,7 +120,7 @@ __device__ __forceinline__ int lm_prefix(int *prefix, int seqs, int *error, F &&
         }
         if (s < seqs) prefix[s] = (int)(before + sum - own);
     }
-    const bool fits = before_all <= 0x7fffffff;
+    const bool fits = before_all < 0x7fffffff;
     if (threadIdx.x == 0) {
         if (!fits) lm_fail(error, LM_TOO_LONG, 0);
         prefix[seqs] = (int)before_all;

@@ -249,7 +249,7 @@ int gpx_count_diff(const void *a, const void *b, size_t bytes, uint64_t *diff, g
  *   2  a page number outside the cache (sequence *where),
  *   3  a position past the rotation table (sequence *where; its new tokens were left out),
  *   4  a bounded wait gave up (CTA *where; the results are incomplete),
- *   5  more work than one launch counts (2^31 - 1 blocks of 64 keys); nothing was done. */
+ *   5  more work than one launch counts (2^31 - 2 blocks of 64 keys); nothing was done. */
 int gpx_lm_ctx_bytes(size_t *bytes);
 int gpx_lm_ctx_reset(void *ctx, gpx_event *ready);
 int gpx_lm_status(const void *ctx, int *error, int *where);

@@ -249,3 +249,24 @@ def test_queries_at_the_ends_of_their_type(gpx, ctx, new, power):
     check(got, ref, weight, dtype, 11, 2.0 ** -13, c, values_largest(bed))
     assert np.all(np.abs(lse - ref_lse) <= 2.0 ** -13)
     bed.free()
+
+
+# ---- more work than a launch counts -------------------------------------------------------------------
+
+@pytest.mark.parametrize("seqs,new,pages_a_seq", [(8, 1, 1 << 13), (4, 1, 1 << 13), (32, 1, 1 << 12), (1, 1, 1 << 15), (1, 33, 1 << 16), (2, 33, 1 << 16)])
+def test_more_work_than_a_launch_counts_is_reported(gpx, seqs, new, pages_a_seq):
+    """Sums over the sequences that pass 31 bits, of one warp's sequences or of one sequence alone: nothing is done.
+    (All sequences have the one page of the cache, again and again.)"""
+    heads, dim, page = 1 << 15, 64, 128
+    mine, cache = gpx.LmContext(), gpx.KvCache(1, page, heads, dim)
+    d = gpx.DeviceBuffer.from_numpy
+    arrays = [d(np.zeros((seqs, pages_a_seq), np.int32)), d(np.full(seqs, pages_a_seq * page, np.int32)), d((np.arange(seqs + 1) * new).astype(np.int32))]
+    batch = gpx.KvBatch(seqs, seqs * new, new, *arrays, pages_a_seq)
+    q, out = gpx.DeviceBuffer(seqs * new * heads * dim * 2), d(np.full(seqs * new * heads * dim, 0x1234, np.uint16))
+    q.zero()
+    gpx.kv_attend(cache, batch, q, out, heads, "bfloat16", mine)
+    gpx.device_sync()
+    assert mine.status() == (5, 0)
+    assert np.all(out.download(np.uint16) == 0x1234)
+    for b in (*arrays, q, out, mine, cache):
+        b.free()
