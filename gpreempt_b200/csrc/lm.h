@@ -24,6 +24,7 @@ namespace gpx {
 constexpr int kLmCounters = 65536;
 constexpr int kLmMaxSeqs = 4096;
 constexpr int kMostPageTokens = 128;
+constexpr int kMostContext = 0x7fffffff - 4096;  // of a sequence: the ends of its last page and of the blocks fetched ahead are still an int
 constexpr size_t kLmResetBytes = 256 + kLmCounters * sizeof(int);
 constexpr size_t kLmPartsOffset = kLmResetBytes + (kLmMaxSeqs + 64) * sizeof(int);
 constexpr size_t kLmPartsBytes = (size_t)64 << 20;
@@ -86,7 +87,7 @@ struct LmSpan {
 __device__ __forceinline__ LmSpan lm_span(const LmBatch &b, int s, int page_tokens, bool new_in_context, int *error) {
     const int f = b.first[s], e = b.first[s + 1], c = b.context[s];
     const bool fine = f >= 0 && e >= f && e <= b.tokens && e - f <= b.most_new && c >= 0 &&
-                      c <= (long long)b.table_ld * page_tokens && (!new_in_context || c >= e - f);
+                      c <= kMostContext && c <= (long long)b.table_ld * page_tokens && (!new_in_context || c >= e - f);
     if (!fine) {
         lm_fail(error, LM_BAD_SPAN, s);
         return {0, 0, 0};

@@ -265,7 +265,7 @@ int gpx_kv_cache_destroy(gpx_kv_cache *cache);
 /* A ragged batch of at most 4096 sequences; the arrays are int32 on the device.  Sequence s has context[s] tokens,
  * the new ones of this step among them, in the pages table[s][0], table[s][1], ... (table_ld page numbers a row);
  * its new tokens are rows first[s] .. first[s + 1] - 1 of the step's tensors (none is allowed) and the last ones of
- * the sequence.  `tokens` rows there are in all, `most_new` of one sequence at most. */
+ * the sequence.  `tokens` rows there are in all, `most_new` of one sequence at most; no sequence is longer than 2^31 - 4097. */
 typedef struct gpx_kv_batch {
     const void *table, *context, *first;
     int table_ld, seqs, tokens, most_new;

@@ -270,3 +270,28 @@ def test_more_work_than_a_launch_counts_is_reported(gpx, seqs, new, pages_a_seq)
     assert np.all(out.download(np.uint16) == 0x1234)
     for b in (*arrays, q, out, mine, cache):
         b.free()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_at_the_end_of_an_int_are_reported(gpx, new):
+    """The places of the last page's end and of what is fetched ahead have to be ints; what does not fit counts as empty."""
+    heads, dim, page, pages_a_seq = 1, 64, 128, 1 << 24
+    mine, cache = gpx.LmContext(), gpx.KvCache(1, page, heads, dim)
+    d = gpx.DeviceBuffer.from_numpy
+    for context in (2 ** 31 - 4096, 2 ** 31 - 64, 2 ** 31 - 1):
+        arrays = [d(np.zeros((1, pages_a_seq), np.int32)), d(np.array([context], np.int32)), d(np.array([0, new], np.int32))]
+        batch = gpx.KvBatch(1, new, new, *arrays, pages_a_seq)
+        x, out = gpx.DeviceBuffer(new * heads * dim * 2), d(np.full(new * heads * dim, 0x1234, np.uint16))
+        x.zero()
+        gpx.kv_attend(cache, batch, x, out, heads, "bfloat16", mine)
+        gpx.device_sync()
+        assert mine.status() == (1, 0)
+        mine.reset()
+        gpx.kv_append(cache, batch, None, x, x, None, heads, "bfloat16", mine)
+        gpx.device_sync()
+        assert mine.status() == (1, 0)
+        mine.reset()
+        assert np.all(out.download(np.uint16) == 0x1234) and not cache.k_scale.download(np.float32).any()
+        for b in (*arrays, x, out):
+            b.free()
+    mine.free(), cache.free()
