@@ -593,6 +593,8 @@ extern "C" int gpx_token_scores(const gpx_token_scores_args *args, void *ctx, co
     GPX_REQUIRE(a.top > 0 || (!a.top_ids && !a.top_logprob), GPX_OUT_OF_RANGE, "top is 0, but its outputs are given");
     GPX_REQUIRE(!a.logprob || a.targets, GPX_FAIL, "logprob needs targets");
     GPX_REQUIRE(a.inv_temperature > 0.f && a.inv_temperature <= 3.4e38f, GPX_OUT_OF_RANGE, "inv_temperature must be positive and finite");
+    GPX_REQUIRE(((uintptr_t)a.targets | (uintptr_t)a.logprob | (uintptr_t)a.entropy | (uintptr_t)a.lse | (uintptr_t)a.top_ids |
+                 (uintptr_t)a.top_logprob) % 4 == 0, GPX_FAIL, "targets and the outputs must be 4-byte aligned");
     p.ld = a.ld ? a.ld : a.vocab;
     GPX_REQUIRE(p.ld >= a.vocab, GPX_OUT_OF_RANGE, "a row of %d is longer than the distance to the next, %lld", a.vocab, p.ld);
     const DeviceInfo &d = device_info();

@@ -313,7 +313,7 @@ int gpx_kv_attend(const gpx_kv_cache *cache, const gpx_kv_batch *batch, const gp
                   const gpx_blp *blp, gpx_stream s);
 
 /* Log probabilities from logits [rows][vocab] ("float32", "bfloat16" or "float16", ld elements from row to row, 0:
- * vocab), each multiplied by inv_temperature (> 0) first.  Any of the outputs may be NULL.
+ * vocab), each multiplied by inv_temperature (> 0) first.  Any of the outputs may be NULL; they and targets are 4-byte aligned.
  *   logprob[row]   of targets[row] (int32; needs targets): 0 for a negative target (no token to score), NaN for one
  *                  at or past vocab;
  *   entropy[row]   of the distribution, in nats;

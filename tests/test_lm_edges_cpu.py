@@ -1,0 +1,23 @@
+"""What the decoder's serving step refuses on the host, and what its example leaves as it was when it refuses."""
+import ctypes
+
+import pytest
+
+from gpreempt_b200 import binding as B
+from gpreempt_b200 import build as gpx_build
+
+
+@pytest.fixture(scope="module")
+def lib():
+    gpx_build.build()
+    return B.load()
+
+
+@pytest.mark.parametrize("name", ["targets", "logprob", "entropy", "lse", "top_ids", "top_logprob"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_scores_refuse_arrays_off_their_boundary(lib, name, off):
+    p = 1 << 20
+    a = B.TokenScoresArgs(logits=p, targets=p, rows=2, vocab=100, top=3, inv_temperature=1.0, dtype=b"float32")
+    setattr(a, name, p + off)
+    assert lib.gpx_token_scores(ctypes.byref(a), ctypes.c_void_p(p), None, None) == B.FAIL
+    assert b"aligned" in lib.gpx_last_error()
