@@ -26,12 +26,17 @@ class Pages:
         self.context = np.zeros(seqs, np.int32)
 
     def grow(self, new) -> np.ndarray:
-        """Makes room for new[s] tokens of each sequence; returns the offsets of the sequences' new tokens."""
+        """Makes room for new[s] tokens of each sequence, or for none of them (MemoryError); returns the offsets of the
+        sequences' new tokens."""
+        need, left = [], len(self.free)
         for s, n in enumerate(new):
             have, want = (-(-int(c) // self.page_tokens) for c in (self.context[s], self.context[s] + n))
-            if want > self.table.shape[1] or want - have > len(self.free):
+            left -= want - have
+            if want > self.table.shape[1] or left < 0:
                 raise MemoryError(f"sequence {s} needs {want - have} more pages")
-            for i in range(have, want):
+            need.append(range(have, want))
+        for s, n in enumerate(new):
+            for i in need[s]:
                 self.table[s, i] = self.free.pop()
             self.context[s] += n
         return np.concatenate([[0], np.cumsum(new)]).astype(np.int32)

@@ -5,6 +5,7 @@ import pytest
 
 from gpreempt_b200 import binding as B
 from gpreempt_b200 import build as gpx_build
+from gpreempt_b200.decode import Pages
 
 
 @pytest.fixture(scope="module")
@@ -21,3 +22,23 @@ def test_scores_refuse_arrays_off_their_boundary(lib, name, off):
     setattr(a, name, p + off)
     assert lib.gpx_token_scores(ctypes.byref(a), ctypes.c_void_p(p), None, None) == B.FAIL
     assert b"aligned" in lib.gpx_last_error()
+
+
+# ---- the example's pages -----------------------------------------------------------------------------
+
+def state_of(p):
+    return p.context.tolist(), p.table.tolist(), list(p.free)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 60], [16, 16, 16], [0, 0, 33], [1, 49, 1]])
+def test_a_refused_step_takes_no_pages(new):
+    """The sequence at fault comes behind others that would have had their pages."""
+    p = Pages(5, 16, 3, 48)
+    p.grow([10, 5, 16])
+    before = state_of(p)
+    with pytest.raises(MemoryError):
+        p.grow(new)
+    assert state_of(p) == before
+    p.release(1)
+    assert p.grow([1, 0, 16]).tolist() == [0, 1, 1, 17]
+    assert p.context.tolist() == [11, 0, 32]
