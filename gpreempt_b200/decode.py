@@ -20,7 +20,7 @@ class Pages:
     """Which pages of a pool hold which sequence: a free list, and a table that grows with the sequences."""
 
     def __init__(self, pages: int, page_tokens: int, seqs: int, most_tokens: int):
-        self.page_tokens = page_tokens
+        self.page_tokens, self.most_tokens = page_tokens, most_tokens
         self.free = list(range(pages - 1, -1, -1))
         self.table = np.full((seqs, -(-most_tokens // page_tokens)), -1, np.int32)
         self.context = np.zeros(seqs, np.int32)
@@ -32,7 +32,9 @@ class Pages:
         for s, n in enumerate(new):
             have, want = (-(-int(c) // self.page_tokens) for c in (self.context[s], self.context[s] + n))
             left -= want - have
-            if want > self.table.shape[1] or left < 0:
+            if self.context[s] + n > self.most_tokens:
+                raise MemoryError(f"sequence {s} has {self.context[s]} tokens of {self.most_tokens}, {n} more do not fit")
+            if left < 0:
                 raise MemoryError(f"sequence {s} needs {want - have} more pages")
             need.append(range(have, want))
         for s, n in enumerate(new):

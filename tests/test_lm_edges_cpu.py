@@ -42,3 +42,17 @@ def test_a_refused_step_takes_no_pages(new):
     p.release(1)
     assert p.grow([1, 0, 16]).tolist() == [0, 1, 1, 17]
     assert p.context.tolist() == [11, 0, 32]
+
+
+@pytest.mark.parametrize("most", [50, 1, 16, 47])
+def test_a_sequence_ends_at_its_most_tokens_not_at_its_last_page(most):
+    """Rotation tables and buffers are made for `most` tokens a sequence; its pages have room for more."""
+    p = Pages(100, 32, 2, most)
+    p.grow([most - 1, 0])
+    before = state_of(p)
+    for new in ([2, 0], [1, most + 1]):
+        with pytest.raises(MemoryError):
+            p.grow(new)
+        assert state_of(p) == before
+    p.grow([1, most])
+    assert p.context.tolist() == [most, most]
