@@ -112,10 +112,12 @@ class Decoder:
         """Takes in tokens[s] (arrays, some may be empty) of every sequence.  Returns for each the log probabilities of its
         tokens behind the first, the entropies behind each token, and the most likely next token (-1 without new ones)."""
         new = [len(t) for t in tokens]
+        ids = np.concatenate([np.asarray(t, np.int64) for t in tokens])
+        if np.any((ids < 0) | (ids >= self.VOCAB)):
+            raise ValueError(f"tokens are 0 to {self.VOCAB - 1}")
         first, rows, h = self.pages.grow(new), sum(new), self.HEADS * self.DIM
         if rows == 0:
             return [np.empty(0, np.float32)] * self.seqs, [np.empty(0, np.float32)] * self.seqs, np.full(self.seqs, -1)
-        ids = np.concatenate([np.asarray(t, np.int64) for t in tokens])
         targets = np.full(rows, -1, np.int32)
         for s in range(self.seqs):
             if new[s] > 1:

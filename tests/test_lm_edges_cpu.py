@@ -1,11 +1,12 @@
 """What the decoder's serving step refuses on the host, and what its example leaves as it was when it refuses."""
 import ctypes
 
+import numpy as np
 import pytest
 
 from gpreempt_b200 import binding as B
 from gpreempt_b200 import build as gpx_build
-from gpreempt_b200.decode import Pages
+from gpreempt_b200.decode import Decoder, Pages
 
 
 @pytest.fixture(scope="module")
@@ -56,3 +57,13 @@ def test_a_sequence_ends_at_its_most_tokens_not_at_its_last_page(most):
         assert state_of(p) == before
     p.grow([1, most])
     assert p.context.tolist() == [most, most]
+
+
+@pytest.mark.parametrize("token", [-1, 4096, 1 << 40])
+def test_a_step_with_a_token_outside_the_vocabulary_changes_nothing(token):
+    d = Decoder.__new__(Decoder)  # (what a step looks at before it asks the device for anything)
+    d.seqs, d.pages, d.embedding = 2, Pages(4, 32, 2, 64), np.zeros((Decoder.VOCAB, 8), np.uint16)
+    before = state_of(d.pages)
+    with pytest.raises(ValueError):
+        d.step([[1, 2], [3, token]])
+    assert state_of(d.pages) == before
