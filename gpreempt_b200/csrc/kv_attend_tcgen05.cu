@@ -86,13 +86,6 @@ struct ManyCtl {
 // Of exponents of 2^20 and more the largest itself: it has no bits for the difference.
 __device__ __forceinline__ float reference_of(float largest) { return fabsf(largest) < 1048576.f ? largest - kLift : largest; }
 
-// The largest of three (one instruction on this architecture).
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
 __device__ __forceinline__ void st_shared_v4(uint32_t to, const uint4 &v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
