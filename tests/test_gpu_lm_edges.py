@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from oracle import lm
-from test_gpu_lm import BITS, Bed, from_bits, run_attention, to_bits
+from test_gpu_lm import BITS, Bed, from_bits, preempted_runs, run_attention, to_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -295,3 +295,83 @@ def test_sequences_at_the_end_of_an_int_are_reported(gpx, new):
         for b in (*arrays, x, out):
             b.free()
     mine.free(), cache.free()
+
+
+# ---- paths that ordinary sizes do not take --------------------------------------------------------------
+
+@pytest.mark.parametrize("seqs", [127, 128, 300])
+@pytest.mark.parametrize("most", [20, 300])
+def test_prompts_of_many_sequences(gpx, ctx, seqs, most):
+    """Sums over more than 127 sequences lie in the context; units of a few blocks are tiles, longer ones are cut."""
+    heads, kv, dim, page, dtype = 8, 2, 64, 32, "bfloat16"
+    new = [(7 * i) % most if i % 5 else 0 for i in range(seqs - 1)] + [most]
+    context = [n + (i * 131) % 2500 for i, n in enumerate(new)]
+    bed = Bed(gpx, new, context, heads, kv, dim, page, seed=seqs).upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), dtype), dtype)
+    got, lse = run_attention(gpx, ctx, bed, q, dtype, heads)
+    for some in (slice(0, 4), slice(seqs - 3, seqs)):
+        rows = slice(bed.first[some.start], bed.first[some.stop])
+        ref, ref_lse, weight = lm.attend(q[rows], bed.k, bed.v, bed.ks, bed.vs, bed.table[some], bed.context[some], bed.first[some.start:some.stop + 1] - rows.start)
+        check(got[rows], ref, weight, dtype, 11, 2.0 ** -13, max(context), values_largest(bed))
+        assert np.all(np.abs(lse[rows] - ref_lse) <= 2.0 ** -13)
+    # (the other kernel, a sequence at a time, on all of the rest)
+    again = np.zeros_like(got)
+    for s in range(seqs):
+        if new[s] == 0:
+            continue
+        arrays = [gpx.DeviceBuffer.from_numpy(a) for a in (bed.table[s:s + 1], bed.context[s:s + 1], np.array([0, new[s]], np.int32))]
+        rows = slice(bed.first[s], bed.first[s + 1])
+        alone = type("Alone", (), {"cache": bed.cache, "tokens": new[s], "dim": dim, "batch": gpx.KvBatch(1, new[s], new[s], *arrays, bed.table.shape[1])})
+        again[rows], _ = run_attention(gpx, ctx, alone, q[rows], dtype, heads)
+        for a in arrays:
+            a.free()
+    # two results within a rounding each, and their factors'
+    assert np.all(np.abs(got - again) <= 2.0 ** -7 * np.abs(again) + 2.0 ** -9 * values_largest(bed))
+    bed.free()
+
+
+@pytest.mark.parametrize("new,context,heads,kv,dim,dtype,causal,window,run_us", [
+    ([5] * 60, [4000 + 31 * i for i in range(60)], 16, 4, 128, "float16", True, 0, 250),      # two tiles of rows
+    ([8] * 60, [4000 + 31 * i for i in range(60)], 16, 4, 64, "bfloat16", True, 3000, 250),   # four
+    ([1] * 64, [6000] * 64, 16, 4, 128, "float16", True, 2500, 100),
+    ([64] * 90, [700] * 90, 16, 8, 64, "bfloat16", True, 0, 100),                            # units that are tiles as they are
+    ([37] * 100, [512] * 100, 12, 12, 64, "float16", False, 0, 100),
+    ([900, 500], [4000, 2500], 16, 4, 128, "float16", True, 0, 200),
+    ([700, 900], [3000, 900], 16, 4, 64, "bfloat16", True, 600, 100),
+    ([300, 700], [3000, 2000], 16, 4, 128, "bfloat16", False, 0, 200),
+    ([40] * 200, [60 + 17 * i for i in range(200)], 8, 2, 64, "bfloat16", True, 0, 100),      # sums in the context
+])
+def test_attention_of_every_kind_drains_and_resumes_bit_identically(gpx, ctx, new, context, heads, kv, dim, dtype, causal, window, run_us):
+    page = 64
+    bed = Bed(gpx, new, context, heads, kv, dim, page, seed=4).upload()
+    q = to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), dtype)
+    dq = gpx.DeviceBuffer.from_numpy(q)
+    out, lse = gpx.DeviceBuffer(bed.tokens * heads * dim * 2), gpx.DeviceBuffer(bed.tokens * heads * 4)
+
+    def fresh():
+        out.zero(), lse.zero()
+
+    want = preempted_runs(gpx, lambda blp, s: gpx.kv_attend(bed.cache, bed.batch, dq, out, heads, dtype, ctx, causal=causal, window=window, lse=lse, blp=blp, stream=s),
+                          lambda: [out.download(np.uint16), lse.download(np.uint32)], fresh, run_us, at_least=1)
+    # a launch without a word gives the same numbers within a rounding of each
+    got, _ = run_attention(gpx, ctx, bed, from_bits(q, dtype), dtype, heads, causal=causal, window=window)
+    other = from_bits(want[0], dtype).reshape(got.shape)
+    assert np.all(np.abs(got - other) <= 2.0 ** (1 - BITS[dtype]) * np.abs(got) + 2.0 ** -9 * values_largest(bed) * (8 if dtype == "bfloat16" else 1))
+    dq.free(), out.free(), lse.free(), bed.free()
+
+
+@pytest.mark.parametrize("new,p_bits", [(1, 20), (5, 20), (32, 20), (40, 11)])
+def test_factors_of_float16_results(gpx, ctx, new, p_bits):
+    """Values of both signs that nearly cancel show the factors' bits: 22 up to 32 rows a head of keys, 11 beyond."""
+    heads, kv, dim, page, dtype = 1, 1, 64, 64, "float16"
+    for c in (2, 3, 5, 33):
+        bed = Bed(gpx, [new], [c], heads, kv, dim, page, seed=c)
+        bed.v[:] = np.where(np.arange(page)[:, None] % 2, 0x7E, 0xFE)  # 448 and -448
+        bed.vs[:], bed.ks[:] = 1.0, 2.0 ** -10
+        bed.upload()
+        q = from_bits(to_bits(bed.rng.standard_normal((new, heads, dim)), dtype), dtype)
+        got, _ = run_attention(gpx, ctx, bed, q, dtype, heads, causal=False)
+        ref, _, weight = lm.attend(q, bed.k, bed.v, bed.ks, bed.vs, bed.table, [c], bed.first, causal=False)
+        # scores below 1: float sums of 64 products, the factor and the exponential are good to 2^-21
+        check(got, ref, weight, dtype, p_bits, 2.0 ** -21, c, 448.0)
+        bed.free()
