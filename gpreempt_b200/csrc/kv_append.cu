@@ -241,8 +241,8 @@ kv_append_one_kernel(const __grid_constant__ AppendParams p, BlpArgs blp) {
 // queries of that head's group.  Keys and values of the tile wait in shared memory between the reduction of their
 // amax and their rounding.  The queries ride along because they turn by the same angles, which are twice their bytes to read
 // (as tiles of their own, in the order of memory, the whole took 147 us against 126 at the time).
-// What bounds it is latency: loads of a row, a barrier, stores, with 24 warps an SM, and 48 million instructions, half of what
-// the time holds.  Eight prompts of 21 700 tokens in all, 32 heads of 128 on 8: 100 us (533 MB, 5.3 TB/s); with 16 warps 117, with
+// What bounds it is latency: loads of a row, a barrier, stores, with 24 warps an SM, and 48 million instructions, which fill 46 %
+// of the issue slots.  Eight prompts of 21 700 tokens in all, 32 heads of 128 on 8: 100 us (533 MB, 5.3 TB/s); with 16 warps 117, with
 // 32 (64 registers) 116, with the rotation's order looked up for each row 119.
 constexpr int kAppendThreads = 256;
 template <int D, bool HALF, int MODE>

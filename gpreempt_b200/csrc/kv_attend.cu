@@ -21,9 +21,9 @@
 // at the end of a unit (a sequence, a head of keys, a block of rows); a fifth keeps the ring of blocks full by TMA,
 // with the table's entries and the scales a batch of blocks ahead.
 //
-// Measured, 32 heads of 128 on 8, bf16: single tokens of 64 sequences over 16 384 keys at most 190 us (6.0 TB/s of 6.5 that a
-// copy reaches), of one over 131 071 keys 54.6 (4.9 TB/s: 148 SMs begin and end together, and the parts' join is 5 600 cycles),
-// five of 16 over 2 000 20.3, of one over 517 9.4, a chain of 16 000 cycles from the sums over the sequences to the join.
+// Measured, 32 heads of 128 on 8, bf16: single tokens of 64 sequences over 16 384 keys at most 195 us (5.9 TB/s of 6.5 that a
+// copy reaches), of one over 131 071 keys 54.5 (4.9 TB/s: 148 SMs begin and end together, and the parts' join is 5 600 cycles),
+// five of 16 over 2 000 21.9, of one over 517 9.1, a chain of 16 000 cycles from the sums over the sequences to the join.
 //
 // Work is cut evenly, whatever the sequences' lengths: the blocks of all units lie on one line, and a tile is
 // an equal piece of it.  A unit that spans several tiles leaves their parts in the context, and the
@@ -686,13 +686,18 @@ static auto attend_instance(int dim, int rows, bool half, F &&f) {
 
 // Rows of a head of keys (its group's heads times the tokens) from which on the other kernel takes over.  This kernel's time grows
 // with the blocks of 32 rows, the other's is that of 256 rows.  This and the other, us, 32 heads of 128 on 8:
-//   rows                           16           32           48           64          128
-//    4 sequences over  2 000   22.0 34.3    32.5 34.4    41.0 34.4    43.5 34.5    44.3 35.3
-//   16 sequences over  2 000   39.6 59.5    64.4 59.2    73.4 56.9    95.9 57.5   135.6 59.8
-//    2 sequences over 20 000   37.7 60.4    61.9 60.6    67.6 61.0    69.1 61.2   110.8 61.9
+//   rows                           16           24           32           48           64          128
+//    4 sequences over  2 000   22.5 34.4    31.8 34.6    34.5 34.4    42.9 34.7    45.4 34.6    47.0 35.4
+//   16 sequences over  2 000   38.9 58.7    57.4 58.5    61.9 58.6    88.0 58.8   106.3 58.6   148.6 59.0
+//    2 sequences over 20 000   39.9 62.1    60.3 62.8    66.6 62.6    74.1 62.9    75.5 63.1   121.5 64.1
+// At 32 rows the other is ahead by up to 6 %; the line stays at the end of this kernel's largest instance, up to which factors of fp16
+// results have 22 bits.  For heads of 128 that instance and the one of two tiles use all 255 registers, and the larger spills 188
+// (bf16) and 236 (fp16) bytes.
 constexpr int kManyRows = 32;
 
-constexpr int kBlocksATile = 16;  // of a preemptible launch: 1024 keys, 256 KiB of a head of 128
+// Of a preemptible launch: 1024 keys, 256 KiB of a head of 128.  64 sequences over 16 384 keys drain in 21 us at the median, 24 at
+// most, and take 257 us on the device; without a word, where a tile is a CTA's whole share, 201.
+constexpr int kBlocksATile = 16;
 
 cudaError_t kv_attend_few_launch(AttendParams &p, int dim, bool half, const DeviceInfo &d, const BlpArgs &blp, cudaStream_t s) {
     const int rows = (int)std::min<long long>((long long)p.batch.most_new * (p.heads / p.kv_heads), 1 << 20);

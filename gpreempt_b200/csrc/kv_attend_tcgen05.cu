@@ -11,18 +11,20 @@
 //   - one warp issues S = Q K^T and O += P V of the two halves of the rows in turn,
 //   - two warpgroups, a thread a row, take the scores out of tensor memory, and put the probabilities back as a 16-bit A
 //     operand, where the scores were.  The values lie with keys as rows; their descriptor names that MN-major.
-// Queries become halves after a power of two that brings their row's largest to 1, as in kv_attend.cu.
+// Queries become halves after a power of two that brings their row's largest to 1, as in kv_attend.cu.  Factors are one half, of fp16
+// results too (kv_attend.cu takes two for those): eleven bits, the result's own; a second product of 128 keys would add half to the tensor cores' time.
 //
 // What bounds it: 256 x 128 exponentials a block are 2 048 cycles of the special-function unit, the products 2 048
 // of the tensor cores, and shared memory carries 320 KB for them (2 500 cycles).  The halves of the rows are
 // half a block apart, so that one's products run under the other's softmax, and a block takes 3 600 cycles: 2 050 from a
 // half's scores to its factors, 1 450 from those to its next scores.  (Four warpgroups for the scores, two threads a row,
 // took as long for the factors and 300 more to agree on them: 391 us against 362.)  The start and end of a unit take another
-// 25 000.  Chunks of 2 048 and 889 tokens over contexts of 8 192 and 3 474, 32 heads of 128 on 8: 323 us (875 TFLOP/s), 2 300
-// with the kernel for few rows.
+// 25 000.  Chunks of 2 048 and 889 tokens over contexts of 8 192 and 3 474, 32 heads of 128 on 8: 321 us (886 TFLOP/s), 2 300
+// with the kernel for few rows.  At 128 registers for the compiler it spills 244 to 320 bytes for heads of 128, 184 to 240 for 64.
 //
 // A tile can last hundreds of microseconds.  The fetching warp reads the preempt word before every block; once it is
-// raised the tile ends behind the blocks under way, sums and statistics go to the context, and the next launch goes on from there.
+// raised the tile ends behind the blocks under way, sums and statistics go to the context, and the next launch goes on from there: drained
+// in 21 us at the median, 23 at most, in the case above, which takes no longer with a word than without.
 #include "act_layout.h"
 #include "kv_attend.h"
 #include "planes.cuh"
@@ -42,8 +44,9 @@ constexpr int kTileRows = 256, kTileKeys = 128;
 constexpr int kRawStages = 2, kKeyBuffers = 2, kValueBuffers = 2;  // (a stage of the ring holds a block's keys or its values)
 constexpr unsigned long long kManyWaitNs = 2000000000ull;
 // A row's exponents refer to kLift below its maximum in the first block it sees (so that thousands of keys that weigh 2^-26 each beside one
-// of that block count: a half ends at 2^-25) until their factors sum to more than this in a block, which a half holds; then the maximum is taken anew and the sums are rescaled.  (Asking for the maximum of every block goes
-// through its scores twice, and a new one among 32 rows, which are rescaled together, comes in most blocks.)
+// of that block count: a half ends at 2^-25) until their factors sum to more than this in a block, which a half holds; then the maximum
+// is taken anew and the sums are rescaled.  (Asking for the maximum of every block goes through its scores twice, and a new one among
+// 32 rows, which are rescaled together, comes in most blocks.  2^7 below and sums up to 2^15 took 327 to 350 us where this takes 317 to 328.)
 constexpr float kMostFactors = 60000.f, kLift = 6.f;
 // What the start of a unit takes (queries, the first blocks until their products run, outputs), in blocks: that many places of the
 // line come before its own, so that a tile of many short units has as long as one of a single long unit.

@@ -18,8 +18,8 @@
 //
 // What bounds it: memory, 2 bytes an element, with the special-function unit (one exponential an element, 16 a cycle
 // and SM) close behind; what it waits for is loads, two kilobytes a warp of which are under way.  4 096 rows of 50 257 fp16: 85 us
-// (4.8 TB/s), 95 with one alternative, 110 with twenty (registers: 16 warps an SM instead of 24; with fewer registers the
-// loop spills, 118 and 138).  64 rows of 131 072 bf16: 11 us, with twenty alternatives 22.
+// (4.8 TB/s), 92 with one alternative, 110 with twenty (registers: 16 warps an SM instead of 24; with fewer registers the
+// loop spills, 118 and 138).  64 rows of 131 072 bf16: 11 us, with twenty alternatives 21.
 #include "act_layout.h"
 #include "lm.h"
 
@@ -622,7 +622,8 @@ extern "C" int gpx_token_scores(const gpx_token_scores_args *args, void *ctx, co
         const long long most = std::max(1ll, std::min((long long)a.vocab * esize / (16 * 32),
                                                       (long long)(kLmPartsBytes / (kScorePartFloats * sizeof(float))) / a.rows));
         if (2ll * a.rows < resident) parts = 2 * resident / 3 / a.rows;
-        // (a launch that can be preempted drains at the end of a unit: 8 192 elements of 24 warps an SM are 9 us)
+        // (a launch that can be preempted drains at the end of a unit; with 8 192 elements, 4 096 rows of 50 257 fp16 with one
+        // alternative drain in 17 us at the median, 20 at most, and take 172 us on the device, 94 without a word)
         if (b.preempted) parts = std::max(parts, (a.vocab + 8191ll) / 8192);
         parts = std::max(1ll, std::min({parts, most, (a.vocab + 1023ll) / 1024}));
     }

@@ -110,7 +110,8 @@ class Decoder:
 
     def step(self, tokens: list) -> tuple:
         """Takes in tokens[s] (arrays, some may be empty) of every sequence.  Returns for each the log probabilities of its
-        tokens behind the first, the entropies behind each token, and the most likely next token (-1 without new ones)."""
+        tokens behind the first, the entropies behind each token, and the most likely next token (-1 without new ones).
+        (Prompts and single tokens share a call here; a server with many of both in a step makes one for each.)"""
         new = [len(t) for t in tokens]
         ids = np.concatenate([np.asarray(t, np.int64) for t in tokens])
         if np.any((ids < 0) | (ids >= self.VOCAB)):
@@ -164,7 +165,7 @@ def main() -> None:
     ap.add_argument("--prompt", type=int, default=100, help="tokens of the longest prompt")
     ap.add_argument("--steps", type=int, default=32)
     ap.add_argument("--window", type=int, default=0)
-    ap.add_argument("--best-effort", action="store_true", help="preemptible launches that poll a preempt word")
+    ap.add_argument("--best-effort", action="store_true", help="preemptible launches (nobody raises their word here: what polling costs)")
     a = ap.parse_args()
     api.init_cuda(0)
     word = api.PreemptWord() if a.best_effort else None
@@ -182,7 +183,7 @@ def main() -> None:
     print(f"prompts: {sum(map(len, prompts))} tokens in {(t1 - t0) * 1e3:.2f} ms, mean log probability {scored.mean() if scored.size else 0.0:.3f}")
     if a.steps > 1:
         print(f"{a.steps - 1} steps of {a.conversations} tokens: {(t2 - t1) / (a.steps - 1) * 1e6:.0f} us a step, "
-              f"mean entropy of the last {np.mean(np.concatenate(entropy)):.3f}, launches interrupted {d.stops}")
+              f"mean entropy of the last {np.mean(np.concatenate(entropy)):.3f}")
     d.free()
 
 

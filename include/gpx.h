@@ -300,7 +300,10 @@ int gpx_kv_append(const gpx_kv_cache *cache, const gpx_kv_batch *batch, const gp
  * With `causal` token i of n new ones in a context of c sees keys 0 .. c - n + i, otherwise all c (cross attention
  * over states that were appended once); with `window` > 0 (causal only) only the last `window` of them.  A row
  * that sees no key is zero, its lse -infinity.  What lies in slots and pages beyond that, NaN codes too, has no
- * influence.  scale 0 stands for 1 / sqrt(head_dim). */
+ * influence.  scale 0 stands for 1 / sqrt(head_dim).
+ * Products are of 16-bit halves with sums in float.  Codes are halves as they are, and so are queries in float16; those in bfloat16
+ * are divided by a power of two of their row (elements 2^-14 and less of the row's largest lose bits).  Probabilities
+ * have eleven bits; in float16, up to 32 rows a head of keys (heads / kv_heads x most_new), 22. */
 typedef struct gpx_kv_attend_args {
     const void *q;
     void *out, *lse;
