@@ -216,7 +216,7 @@ kv_attend_many_kernel(const __grid_constant__ AttendParams p, BlpArgs blp) {
                         atomicCAS(blp.stop_index, -1, blp.kernel_id);
                     } else {
                         t = pending, done = note[1], spilled = note[2];
-                        note[0] = 0;
+                        note[0] = note[1] = note[2] = 0;  // (other kernels' counters and notes are the same words: a note that is taken leaves none behind)
                     }
                     pending = -1;
                 } else {

@@ -127,7 +127,7 @@ kv_weigh_many_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
                     atomicCAS(blp.stop_index, -1, blp.kernel_id);
                 } else {
                     tile = pending, resume = note[1];
-                    note[0] = 0;
+                    note[0] = note[1] = 0;  // (other kernels' counters and notes are the same words: a note that is taken leaves none behind)
                 }
                 pending = -1;
             } else {

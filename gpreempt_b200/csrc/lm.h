@@ -19,8 +19,9 @@ namespace gpx {
 
 // ---- scratch context ------------------------------------------------------------------------------
 
-// Header, arrival counters (zero between launches: whoever joins the parts of a result puts its counter back), and
-// what CTAs have in common: sums over the sequences of a batch, parts of results.
+// Header, arrival counters (zero between launches: whoever joins the parts of a result puts its counter back, and whoever takes
+// a note of an unfinished tile puts back all of its words), and what CTAs have in common: sums over the sequences of a batch,
+// parts of results.
 constexpr int kLmCounters = 65536;
 constexpr int kLmMaxSeqs = 4096;
 constexpr int kMostPageTokens = 128;
