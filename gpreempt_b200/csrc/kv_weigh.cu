@@ -79,6 +79,7 @@ kv_weigh_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
             const int slot = p.account.slots ? p.account.slots[s] : s;
             float *const account = p.account.weights + ((long long)slot * p.kv_heads + head) * p.account.ld;
             const int fresh = p.causal ? max(0, context - n) : context;  // keys from here on begin their account
+            const int seen = p.window && context - votes >= p.window ? context - votes - p.window + 1 : 0;  // the first key that a row sees (and those up to the last one are seen)
             for (int row0 = 0; row0 < rows; row0 += ROWS) {
                 const int some_rows = min(ROWS, rows - row0);
                 auto position = [&](int r) { return context - votes + (row0 + r) / group; };  // (of the rows r of this pass)
@@ -87,8 +88,8 @@ kv_weigh_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
                 // keys that some row sees, and those that every row sees
                 const int pos0 = position(0), pos1 = position(some_rows - 1);
                 const int low = from(pos0), high = upto(pos1), all_low = from(pos1), all_high = upto(pos0);
-                // what a lane knows of the sixteen keys of its warp in block b0 + lane: row of the cache's codes (-1: nobody
-                // sees them, -2: their accounts stay as they are)
+                // what a lane knows of the sixteen keys of its warp in block b0 + lane: row of the cache's codes (-1: no row of this pass
+                // sees them, -2: of no page, and the accounts of those that a row of any pass sees stay as they are)
                 int at_row = -2;
                 float at_scale = 0.f;
                 auto look_up = [&](int b0) {
@@ -96,15 +97,15 @@ kv_weigh_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
                     const int key = (block0 + b0 + lane) * kWeighKeys + wid * 16;
                     if (b0 + lane >= blocks || key >= context) return;
                     at_row = -1;
-                    if (key >= high || key + 16 <= low) return;
+                    if (key + 16 <= seen) return;  // (what ends below may be anybody's by now: its page is not looked up)
                     const int page = p.batch.table[(size_t)s * p.batch.table_ld + (key >> p.page_shift)];
-                    if ((unsigned)page < (unsigned)p.pages) {
+                    if ((unsigned)page >= (unsigned)p.pages) {
+                        lm_fail(p.error, LM_BAD_PAGE, s);
+                        at_row = -2;
+                    } else if (key < high && key + 16 > low) {
                         const long long block = (long long)page * p.kv_heads + head;
                         at_row = (int)((block << p.page_shift) + (key & (page_tokens - 1)));
                         at_scale = p.k_scale[block];
-                    } else {
-                        lm_fail(p.error, LM_BAD_PAGE, s);
-                        at_row = -2;
                     }
                 };
                 struct Keys {
@@ -121,7 +122,7 @@ kv_weigh_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
                         k.b[c] = row >= 0 && b < 32 ? load_codes(codes + 8 * D + 64 * c) : make_uint4(0, 0, 0, 0);
                     }
                     const int key = (block0 + b0 + b) * kWeighKeys + wid * 16 + g + 8 * t;
-                    k.old = t < 2 && b < 32 && row != -2 && key < context && (key < fresh || row0 > 0) ? account[key] : 0.f;
+                    k.old = t < 2 && b < 32 && (row != -2 || key < seen) && key < context && (key < fresh || row0 > 0) ? account[key] : 0.f;
                     return k;
                 };
                 look_up(0);
@@ -197,7 +198,7 @@ kv_weigh_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
                         }
                     }
                     const int key = key0 + g + 8 * t;
-                    if (t >= 2 || row == -2 || key >= context) return;
+                    if (t >= 2 || key >= context || (row == -2 && key >= seen)) return;
                     const float add = t ? sum[1] : sum[0];
                     if (row0 > 0) {
                         if (row >= 0) account[key] = old + add;

@@ -373,9 +373,10 @@ typedef struct gpx_kv_weights {
  * where the rows are the heads that share the key's head, for the last `observed` new tokens of the sequence (0: all).  q, q_ld,
  * heads, causal, window, scale and dtype are what gpx_kv_attend took, lse [token][heads] what it left.  Without `causal` the new
  * tokens are not among the keys, and every account goes on.  Sequences without new tokens keep their accounts as they are, and so
- * do keys whose page is outside the cache.  decay is above 0 and at most 1.  Sums are float, in an order that does not depend
- * on the launch; queries as products see them are those of gpx_kv_attend.  A key whose score is not a number for a row
- * that sees it has an account that is not a number; rows that do not see it have no influence. */
+ * do keys that some of these rows see and whose page is outside the cache (code 2); pages of keys that none sees are not looked
+ * up.  decay is above 0 and at most 1.  Sums are float, in an order that does not depend on the launch; queries as products see
+ * them are those of gpx_kv_attend.  A key whose score is not a number for a row that sees it has an account that is not a
+ * number; rows that do not see it have no influence. */
 typedef struct gpx_kv_weigh_args {
     const void *q, *lse;
     long long q_ld;

@@ -189,3 +189,46 @@ def test_pages_below_a_window_are_not_looked_up(gpx, ctx, new, heads, decay):
         assert ctx.status() == (0, 0)
         free(account, dq, dl)
     bed.free()
+
+
+@pytest.mark.parametrize("decay", [1.0, 0.5])
+@pytest.mark.parametrize("case", [
+    # new, context, page, window, observed; heads share keys four by four
+    (1, 300, 16, 0, 0), (8, 300, 16, 0, 0),  # one pass over the rows
+    (13, 300, 16, 0, 0), (16, 40, 16, 0, 0),  # two: a new token's key may be seen by rows of the second alone
+    (13, 300, 64, 70, 0), (16, 500, 128, 100, 9), (16, 300, 32, 5, 12),  # a window's border in the middle of a page
+    (20, 300, 16, 0, 0), (40, 300, 128, 33, 0), (90, 333, 64, 0, 30),  # many rows
+], ids=lambda c: "%d-%d-p%d-w%d-o%d" % c)
+def test_keys_of_pages_outside_the_cache_keep_their_accounts(gpx, case, decay):
+    """Those that some row sees, however many rows there are and whichever of them see the key; the others fade as any do."""
+    new, c, page, window, observed = case
+    heads, kv, dim, dtype, context = 8, 2, 64, "bfloat16", [c, c - 7]
+    mine = gpx.LmContext()
+    bed = Bed(gpx, [new, new], context, heads, kv, dim, page, seed=6).upload()
+    q = from_bits(to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), dtype), dtype)
+    dq, dl = up(gpx, to_bits(q, dtype)), up(gpx, normalisers(q, bed, context, True, window))
+    lse = dl.download(np.float32).reshape(-1, heads)
+    account = Account(gpx, bed)
+    want, bound = lm.weigh(account.w, account.slots, q, lse, bed.k, bed.ks, bed.table, context, bed.first, None, True, window, observed, decay)
+    votes = observed or new
+    for s, n in enumerate(context):
+        seen = max(0, n - votes + 1 - window) if window else 0
+        last = (n - 1) // page
+        for bad in sorted({seen // page, (n - new) // page, last // 2, last - 1, last} - {-1}):
+            table = bed.table.copy()
+            table[s, bad] = (-1, bed.pages, 2 ** 31 - 1, -2 ** 31)[(bad + s) % 4]
+            bed.arrays[0].upload(table)
+            account.dw.upload(account.w)
+            gpx.kv_weigh(bed.cache, bed.batch, dq, dl, account.handle, heads, dtype, mine, window=window, observed=observed, decay=decay)
+            gpx.device_sync()
+            keys = slice(max(seen, bad * page), min(n, (bad + 1) * page))
+            row = account.slots[s]
+            expected, size = want.copy(), bound.copy()
+            expected[row, :, keys], size[row, :, keys] = account.w[row, :, keys], 0
+            got = account.read()
+            assert np.array_equal(got[row, :, keys], account.w[row, :, keys]), (s, bad)
+            check_weights(got, expected, size, account.w)
+            assert mine.status() == ((2, s) if keys.start < keys.stop else (0, 0))
+            mine.reset()
+    mine.free()
+    free(dq, dl, account, bed)
