@@ -7,7 +7,8 @@ import pytest
 
 from oracle import lm
 from test_gpu_lm import Bed, from_bits, tables, to_bits
-from test_gpu_lm_memory import Account, Moved, assert_codes, check_products, check_weights, free, normalisers, products, up, weights4
+from test_gpu_lm_memory import (KINDS, Account, Moved, assert_codes, check_products, check_weights, free, normalisers, products, up, weights4,
+                                weights_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -232,3 +233,32 @@ def test_keys_of_pages_outside_the_cache_keep_their_accounts(gpx, case, decay):
             mine.reset()
     mine.free()
     free(dq, dl, account, bed)
+
+
+@pytest.mark.parametrize("keep,first,last", [(3000, 2, 100), (18000, 5, 0), (16390, 0, 7000)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_batches_of_accounts_that_shared_memory_does_not_hold(gpx, ctx, kind, keep, first, last):
+    """More accounts than a B200 has SMs, of more entries than 512 threads keep at once: they are read in pieces, and equal weights are
+    counted across the ends of the pieces."""
+    kv = 8
+    context = [33000, 16384 + first + last, 16385 + first + last, 32768 + first + last, 32769 + first + last, 16383, 20000, 24001, 17, 3001,
+               0, 31999, 18000, 18001, 16391, 25000, 30011, 19999, 28672, 1]
+    context = [min(c, 33000) for c in context]
+    rng = np.random.default_rng(keep)
+    rows, ld = len(context) + 1, 33001
+    w = weights_of(kind, (rows, kv, ld), rng)
+    slots = rng.permutation(rows)[:len(context)].astype(np.int32)
+    arrays = [up(gpx, a) for a in (np.full((len(context), 1), -9, np.int32), np.array(context, np.int32), np.full(len(context) + 1, -5, np.int32))]
+    batch = gpx.KvBatch(len(context), 0, 0, *arrays, 1)
+    dw, ds = up(gpx, w), up(gpx, slots)
+    account = gpx.KvWeights(dw, rows, kv, ld, ds)
+    kept, counts = up(gpx, np.full((len(context), kv, keep), -3, np.int32)), up(gpx, np.full(len(context), -3, np.int32))
+    gpx.kv_choose(batch, account, kept, counts, keep, ctx, first=first, last=last)
+    gpx.device_sync()
+    got = kept.download(np.int32).reshape(len(context), kv, keep)
+    assert counts.download(np.int32).tolist() == [min(c, keep) for c in context]
+    for s, want in enumerate(lm.choose(w, slots, context, keep, first, last)):
+        n = want.shape[1]
+        assert np.array_equal(got[s, :, :n], want) and np.all(got[s, :, n:] == -3), s
+    assert ctx.status() == (0, 0)
+    free(dw, ds, kept, counts, *arrays)

@@ -1,12 +1,12 @@
-"""Serving in bounded memory, stopped where work is under way: tiles of accounts that stop between two chunks of rows.  A stop counts here only
-if the launch had begun."""
+"""Serving in bounded memory, stopped where work is under way: launches that have run tiles and have some left, tiles of accounts that stop
+between two chunks of rows, rows of products whose parts were brought by different launches.  A stop counts here only if the launch had begun."""
 import time
 
 import numpy as np
 import pytest
 
-from test_gpu_lm import Bed, to_bits
-from test_gpu_lm_memory import Account, free, up
+from test_gpu_lm import Bed, tables, to_bits
+from test_gpu_lm_memory import Account, Moved, free, up, weights_of
 
 pytestmark = pytest.mark.gpu
 
@@ -126,3 +126,85 @@ def test_accounts_behind_attention_that_was_stopped(gpx, dtype):
     assert not notes(mine).any() and not joins(mine).any()
     word.destroy()
     free(mine, other, dq, out, lse, account, bed)
+
+
+@pytest.mark.parametrize("rows,group,zeros", [(1, 64, False), (24, 32, True), (64, 128, True)])
+def test_rows_of_products_whose_parts_two_launches_bring(gpx, ctx, rows, group, zeros):
+    n, k = 30011, 16384
+    rng = np.random.default_rng(1)
+    codes, scales = up(gpx, rng.integers(0, 256, (n, k // 2), np.uint8)), up(gpx, to_bits(rng.random((n, k // group)) * 0.02, "bfloat16"))
+    z = up(gpx, rng.integers(0, 16, (n, k // group)).astype(np.uint8)) if zeros else None
+    w = gpx.FourBit(codes, scales, z, n, k, group, "bfloat16")
+    x, y = up(gpx, to_bits(rng.standard_normal((rows, k)), "bfloat16")), gpx.DeviceBuffer(rows * n * 2)
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.w4_matvec(w, x, y, rows, ctx, blp=blp, stream=s), lambda: [y.download(np.uint16)], y.zero,
+                 100 if rows == 1 else 200, lambda ctx: joins(ctx).any())
+    free(codes, scales, w, x, y, *([z] if zeros else []))
+
+
+@pytest.mark.parametrize("new,seqs,context", [(1, 40, 10000), (12, 20, 20000)])
+def test_accounts_of_few_rows_stop_between_tiles(gpx, ctx, new, seqs, context):
+    heads, kv, dim, page = 16, 4, 128, 64
+    bed = Bed(gpx, [new] * seqs, [context - 31 * i for i in range(seqs)], heads, kv, dim, page, seed=4).upload()
+    dq, lse = up(gpx, to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), "bfloat16")), up(gpx, np.full((bed.tokens, heads), 9, np.float32))
+    account = Account(gpx, bed)
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.kv_weigh(bed.cache, bed.batch, dq, lse, account.handle, heads, "bfloat16", ctx, decay=0.9, blp=blp, stream=s),
+                 lambda: [account.read()], lambda: account.dw.upload(account.w), 80)
+    free(dq, lse, account, bed)
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+@pytest.mark.parametrize("seqs,most", [(100, 20000), (14, 60000)])
+def test_choosing_stops_between_tiles(gpx, ctx, kind, seqs, most):
+    """Accounts that are read in pieces, more of them than are looked at at once; and few with 1 024 threads each, of which all have begun
+    before a stop can be seen."""
+    kv, keep = 8, 4000
+    context = np.array([most - 30 * i for i in range(seqs)], np.int32)
+    w = up(gpx, weights_of(kind, (seqs, kv, most), np.random.default_rng(2)))
+    arrays = [up(gpx, a) for a in (np.zeros((seqs, 1), np.int32), context, np.zeros(seqs + 1, np.int32))]
+    batch, account = gpx.KvBatch(seqs, 0, 0, *arrays, 1), gpx.KvWeights(w, seqs, kv, most)
+    kept, counts = gpx.DeviceBuffer(seqs * kv * keep * 4), gpx.DeviceBuffer(seqs * 4)
+    few = seqs * kv <= 148
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.kv_choose(batch, account, kept, counts, keep, ctx, 4, 100, blp=blp, stream=s),
+                 lambda: [kept.download(np.int32), counts.download(np.int32)], lambda: (kept.zero(), counts.zero()), 10 if few else 120,
+                 enough=0 if few else 3, trials=12 if few else 60)
+    free(w, kept, counts, *arrays)
+
+
+def test_moving_stops_between_tiles(gpx, ctx):
+    seqs, kv, dim, page, keep = 40, 8, 64, 64, 3000
+    bed = Bed(gpx, [0] * seqs, [6000 - 30 * i for i in range(seqs)], kv, kv, dim, page, seed=4).upload()
+    lists = np.sort(bed.rng.random((seqs, kv, 4800)).argsort(2)[:, :, :keep].astype(np.int32), 2)
+    kept, counts = up(gpx, lists), up(gpx, np.full(seqs, keep, np.int32))
+    account, to, to_account = Account(gpx, bed), Moved(gpx, bed, [keep] * seqs, 16), Account(gpx, bed, seed=5)
+
+    def fresh():
+        for b, a in zip(to.buffers, (to.k, to.v, to.ks, to.vs)):
+            b.upload(a)
+        to_account.dw.upload(to_account.w)
+
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.kv_move(bed.cache, bed.batch, to.cache, to.dt, to.table.shape[1], kept, counts, keep, ctx,
+                                                      account.handle, to_account.handle, blp=blp, stream=s),
+                 lambda: [*to.download(), to_account.read()], fresh, 80)
+    free(kept, counts, account, to_account, to, bed)
+
+
+def test_append_at_stops_between_tiles(gpx, ctx):
+    new, heads, kv, dim, page = [6000, 5000, 8000], 8, 8, 128, 64
+    context = [n + 77 for n in new]
+    bed = Bed(gpx, new, context, heads, kv, dim, page, seed=6).upload()
+    x = up(gpx, to_bits(bed.rng.standard_normal((bed.tokens, 3 * heads * dim)), "bfloat16"))
+    q, width = gpx.DeviceBuffer(bed.tokens * heads * dim * 2), 3 * heads * dim
+    cos, sin = tables(4001, dim)
+    dcos, dsin, dat = up(gpx, cos), up(gpx, sin), up(gpx, bed.rng.integers(0, 4001, (bed.tokens, 3)).astype(np.int32))
+    rope, where = gpx.Rope(dcos, dsin, 4001, dim), gpx.KvPositions(dat, 3, np.arange(dim // 2) % 3)
+
+    def fresh():
+        q.zero()
+        for b, a in ((bed.dk, bed.k), (bed.dv, bed.v), (bed.dks, bed.ks), (bed.dvs, bed.vs)):
+            b.upload(a)
+
+    at = x.ptr.value
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.kv_append_at(bed.cache, bed.batch, at, at + 2 * heads * dim, at + 4 * heads * dim, q, heads, "bfloat16",
+                                                           ctx, rope, where, blp, s, width, width, width),
+                 lambda: [q.download(np.uint16), *bed.download()], fresh, 120)
+    free(x, q, dcos, dsin, dat, bed)
