@@ -27,6 +27,7 @@ class Pages:
         self.free = list(range(pages - 1, -1, -1))
         self.table = np.full((seqs, -(-most_tokens // page_tokens)), -1, np.int32)
         self.context = np.zeros(seqs, np.int32)
+        self.seen = np.zeros(seqs, np.int64)  # tokens that a sequence has had, whatever it has dropped of them
 
     def grow(self, new) -> np.ndarray:
         """Makes room for new[s] tokens of each sequence, or for none of them (MemoryError); returns the offsets of the
@@ -44,6 +45,7 @@ class Pages:
             for i in need[s]:
                 self.table[s, i] = self.free.pop()
             self.context[s] += n
+            self.seen[s] += n
         return np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
 
     def take(self, tokens: int) -> list:
@@ -55,14 +57,16 @@ class Pages:
 
     def replace(self, s: int, pages: list, tokens: int) -> None:
         """A sequence gives back its pages and goes on with others."""
+        seen = self.seen[s]
         self.release(s)
         self.table[s, :len(pages)] = pages
-        self.context[s] = tokens
+        self.context[s], self.seen[s] = tokens, seen
 
     def release(self, s: int) -> None:
+        """A sequence ends: its pages are free, and the next one in its place begins at position 0."""
         used = -(-int(self.context[s]) // self.page_tokens)
         self.free.extend(int(p) for p in self.table[s, :used])
-        self.context[s] = 0
+        self.context[s] = self.seen[s] = 0
 
 
 def _bf16(x: np.ndarray) -> np.ndarray:
@@ -83,7 +87,7 @@ class Decoder:
         if keep and keep < 2 * self.FIRST:
             raise ValueError(f"a conversation keeps {2 * self.FIRST} tokens at least")
         h, self.seqs, self.most_tokens, self.window = self.HEADS * self.DIM, seqs, most_tokens, window
-        self.keep, self.evicted, self.seen = keep, 0, np.zeros(seqs, np.int64)
+        self.keep, self.evicted = keep, 0
         rng = np.random.default_rng(seed)
         self.width = (self.HEADS + 2 * self.KV_HEADS) * self.DIM
         upload = api.DeviceBuffer.from_numpy
@@ -95,6 +99,7 @@ class Decoder:
         # (what is kept moves to pages of its own before the old ones are free)
         pages = seqs * -(-room // self.PAGE) + (seqs * -(-keep // self.PAGE))
         self.pages = Pages(pages, self.PAGE, seqs, room)
+        self.seen = self.pages.seen
         self.cache = api.KvCache(pages, self.PAGE, self.KV_HEADS, self.DIM)
         half = self.DIM // 2
         angle = np.arange(most_tokens)[:, None] * 10000.0 ** (-np.arange(half) / half)
@@ -182,7 +187,7 @@ class Decoder:
         self._gemm(0, self.x, self.w_qkv, self.qkv, rows, self.width)
         if self.keep:
             # a token's position is its number in the conversation, whatever has been dropped of it
-            self.at.upload(np.concatenate([np.arange(p, p + n) for p, n in zip(self.seen, new)]).astype(np.int32), s)
+            self.at.upload(np.concatenate([np.arange(p - n, p) for p, n in zip(self.seen, new)]).astype(np.int32), s)
             where = api.KvPositions(self.at)
             self._run(lambda: api.kv_append_at(self.cache, batch, at, k, v, self.q, self.HEADS, bf, self.ctx, self.rope, where, self.blp, s, self.width,
                                                self.width, self.width))
@@ -198,7 +203,6 @@ class Decoder:
         self._gemm(2, self.y, self.w_head, self.logits, rows, self.VOCAB)
         self._run(lambda: api.token_scores(self.logits, rows, self.VOCAB, bf, self.ctx, self.targets, self.logprob, self.entropy, top=1,
                                            top_ids=self.best, blp=self.blp, stream=s))
-        self.seen += new
         if self.keep:
             self._evict([i for i in range(self.seqs) if self.pages.context[i] >= 2 * self.keep])
         s.sync()

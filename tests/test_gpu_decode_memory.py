@@ -152,3 +152,24 @@ def test_a_best_effort_decoder_in_bounded_memory_under_interruptions(gpx):
     for a, b in zip(got, want):
         assert np.array_equal(a, b)
     word.destroy()
+
+
+def test_a_conversation_that_has_ended_leaves_its_place_as_it_was(gpx):
+    """After evictions and the end of all conversations the next ones come to the bits of a decoder that has had none."""
+    from gpreempt_b200.decode import Decoder
+
+    rng = np.random.default_rng(8)
+    before, after = ([rng.integers(0, Decoder.VOCAB, n) for n in lengths] for lengths in ((50, 30, 9), (20, 48, 33)))
+    fresh = Decoder(3, 150, keep=24, room=60)
+    want = _decode(fresh, after, 60)
+    fresh.free()
+    d = Decoder(3, 150, keep=24, room=60)
+    _decode(d, before, 60)
+    assert d.evicted >= 3
+    for s in range(3):
+        d.pages.release(s)
+    got = _decode(d, after, 60)
+    assert d.seen.tolist() == [80, 108, 93]
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
+    d.free()

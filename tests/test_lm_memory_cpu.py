@@ -231,3 +231,21 @@ def test_the_restatement_of_choosing_and_moving():
     got = [got[1, 0, 0], got[1, 0, 1], got[1, 0, 2], got[1, 0, 3], got[0, 0, 0]]
     for a, b in zip(got, want):
         assert np.all(np.abs(a - b) <= np.maximum(np.abs(b) * 2.0 ** -4, 2.0 ** -10 * to_scale.max()))
+
+
+def test_a_sequence_that_ends_leaves_no_positions_behind():
+    from gpreempt_b200.decode import Pages
+
+    p = Pages(8, 16, 2, 64)
+    p.grow([20, 5])
+    p.grow([1, 0])
+    assert p.seen.tolist() == [21, 5]
+    p.replace(0, p.take(7), 7)  # an eviction: its next token is still its 22nd
+    assert p.context.tolist() == [7, 5] and p.seen.tolist() == [21, 5]
+    with pytest.raises(MemoryError):
+        p.grow([1, 60])
+    assert p.seen.tolist() == [21, 5]
+    p.release(0)
+    assert p.context.tolist() == [0, 5] and p.seen.tolist() == [0, 5]
+    p.grow([3, 1])
+    assert p.seen.tolist() == [3, 6] and len(p.free) == 6
