@@ -76,8 +76,8 @@ def _bf16(x: np.ndarray) -> np.ndarray:
 
 class Decoder:
     """Weights, cache and buffers of a tenant; `word` makes its launches preemptible.  With `keep` a conversation of 2 x keep tokens and
-    more keeps that many behind a step, and `room` is how many it may hold at once (most_tokens: all); with `four_bit` steps of a few
-    tokens read weights of 4 bits."""
+    more keeps that many behind a step, and `room` is how many it may hold at once (0: most_tokens; not below 2 x keep, where it would never
+    drop any); with `four_bit` steps of a few tokens read weights of 4 bits."""
 
     HEADS, KV_HEADS, DIM, PAGE, VOCAB, TILE = 8, 2, 64, 32, 4096, 128
     GROUP, FIRST = 64, 4  # elements that have one scale; tokens at the start of a conversation that it always keeps
@@ -86,6 +86,9 @@ class Decoder:
                  room: int = 0, four_bit: bool = False):
         if keep and keep < 2 * self.FIRST:
             raise ValueError(f"a conversation keeps {2 * self.FIRST} tokens at least")
+        room = room or most_tokens
+        if keep and room < min(2 * keep, most_tokens):
+            raise ValueError(f"with room for {room} tokens a conversation does not get to the {2 * keep} of which it keeps {keep}")
         h, self.seqs, self.most_tokens, self.window = self.HEADS * self.DIM, seqs, most_tokens, window
         self.keep, self.evicted = keep, 0
         rng = np.random.default_rng(seed)
@@ -95,7 +98,6 @@ class Decoder:
         weights = [rng.standard_normal((n, h)) * s / h ** 0.5 for n, s in ((self.width, 1.5), (h, 1.0), (self.VOCAB, 2.0))]
         self.w_qkv, self.w_out, self.w_head = (upload(_bf16(w)) for w in weights)
         self.w4 = [self._four_bit(w) for w in weights] if four_bit else None
-        room = room or most_tokens
         # (what is kept moves to pages of its own before the old ones are free)
         pages = seqs * -(-room // self.PAGE) + (seqs * -(-keep // self.PAGE))
         self.pages = Pages(pages, self.PAGE, seqs, room)

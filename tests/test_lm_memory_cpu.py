@@ -249,3 +249,12 @@ def test_a_sequence_that_ends_leaves_no_positions_behind():
     assert p.context.tolist() == [0, 5] and p.seen.tolist() == [0, 5]
     p.grow([3, 1])
     assert p.seen.tolist() == [3, 6] and len(p.free) == 6
+
+
+@pytest.mark.parametrize("keep,room", [(50, 60), (50, 99), (24, 1), (60, 100)])
+def test_a_decoder_without_room_to_grow_to_an_eviction_is_refused(keep, room):
+    """Before anything is asked of a GPU."""
+    from gpreempt_b200.decode import Decoder
+
+    with pytest.raises(ValueError, match="room"):
+        Decoder(1, 200, keep=keep, room=room)
