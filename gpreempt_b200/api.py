@@ -503,19 +503,32 @@ def kv_move(cache: KvCache, batch: KvBatch, to: KvCache, to_table, to_ld: int, k
              to_account._ref if to_account is not None else None)
 
 
-def quantize_w4(weights, group: int, zeros: bool = True):
-    """Codes, scales (float) and zeros (None without) of weights [n][k] in 4 bits, each group of a row by its own range."""
+def quantize_w4(weights, group: int, zeros: bool = True, dtype: str = "bfloat16"):
+    """Codes, scales (float) and zeros (None without) of weights [n][k] in 4 bits, each group of a row by its own range.  Scales are numbers that
+    `dtype` has, in which the products read them, and codes are rounded by those (scales of a type with fewer bits would be other steps: up to
+    2^-9 of the fifteen)."""
     w = np.asarray(weights, np.float32)
     n, k = w.shape
     if group not in (32, 64, 128) or k % group:
         raise ValueError(f"{k} elements of a row in groups of {group}")
+    if dtype not in ("bfloat16", "float16"):
+        raise ValueError(f"scales are bfloat16 or float16, not {dtype}")
     g = w.reshape(n, k // group, group)
+    low, high = np.minimum(g.min(2), 0), np.maximum(g.max(2), 0)
+    scale = (high - low) / 15 if zeros else np.maximum(high, -low) / 7
+    if dtype == "float16":
+        with np.errstate(over="ignore"):
+            scale = scale.astype(np.float16).astype(np.float32)
+    else:
+        u = np.ascontiguousarray(scale, np.float32).view(np.uint32)
+        scale = ((u + 0x7FFF + (u >> 16 & 1)) & 0xFFFF0000).astype(np.uint32).view(np.float32)
+    if not np.all(np.isfinite(scale)):
+        raise ValueError(f"a group of weights has no scale in {dtype}")
+    smallest = np.float32(2.0 ** (-24 if dtype == "float16" else -133))
+    scale = np.where(high > low, np.maximum(scale, smallest), np.float32(1))
     if zeros:
-        low, high = np.minimum(g.min(2), 0), np.maximum(g.max(2), 0)
-        scale = np.where(high > low, (high - low) / 15, 1).astype(np.float32)
         zero = np.clip(np.rint(-low / scale), 0, 15).astype(np.uint8)
     else:
-        scale = np.where(np.abs(g).max(2) > 0, np.abs(g).max(2) / 7, 1).astype(np.float32)
         zero = np.full(scale.shape, 8, np.uint8)
     q = np.clip(np.rint(g / scale[:, :, None]) + zero[:, :, None], 0, 15).astype(np.uint8).reshape(n, k)
     return q[:, 0::2] | q[:, 1::2] << 4, scale, zero if zeros else None

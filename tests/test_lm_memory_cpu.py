@@ -258,3 +258,46 @@ def test_a_decoder_without_room_to_grow_to_an_eviction_is_refused(keep, room):
 
     with pytest.raises(ValueError, match="room"):
         Decoder(1, 200, keep=keep, room=room)
+
+
+def _held_by(x, dtype):
+    """x as the products read scales of this type."""
+    if dtype == "float16":
+        return x.astype(np.float16).astype(np.float64)
+    u = x.astype(np.float32).view(np.uint32).astype(np.int64)
+    return (((u + 0x7FFF + (u >> 16 & 1)) >> 16 << 16).astype(np.uint32)).view(np.float32).astype(np.float64)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("zeros", [True, False])
+def test_codes_belong_to_the_scales_that_the_products_read(zeros, dtype):
+    """Codes that are not the outermost ones are within half a step of the 16-bit scale; a division and a product are rounded to 2^-24 of at
+    most fifteen steps each."""
+    from gpreempt_b200 import api
+
+    w = np.random.default_rng(3).standard_normal((64, 1024)).astype(np.float32)
+    w[1] *= 1e-9 if dtype == "float16" else 1e-38  # scales where the type runs out of numbers
+    w[2] = 0
+    w[3, :128], w[3, 64] = 0, 1e-45
+    with np.errstate(all="raise", under="ignore"):
+        codes, scales, zero = api.quantize_w4(w, 128, zeros, dtype=dtype)
+    assert scales.dtype == np.float32 and np.array_equal(scales, _held_by(scales, dtype)) and np.all(scales > 0)
+    q = np.stack([codes & 15, codes >> 4], 2).reshape(64, 8, 128).astype(np.float64)
+    offset = 8.0 if zero is None else zero[:, :, None].astype(np.float64)
+    steps = np.abs(w.reshape(64, 8, 128) / scales[:, :, None].astype(np.float64) - (q - offset))
+    inner = (q > 0) & (q < 15)
+    assert np.max(steps[inner]) <= 0.5 + 30 * 2.0 ** -24 and np.max(steps) <= 0.51 + 0.5 * zeros
+    back = lm.w4_weights(codes, scales, zero, 128)
+    assert np.all(back[2] == 0)
+
+
+def test_weights_without_a_scale_are_refused():
+    from gpreempt_b200 import api
+
+    for value, dtype in ((np.nan, "bfloat16"), (np.inf, "float16"), (1e7, "float16")):
+        w = np.ones((2, 64), np.float32)
+        w[1, 5] = value
+        with pytest.raises(ValueError, match="scale"):
+            api.quantize_w4(w, 32, dtype=dtype)
+    with pytest.raises(ValueError, match="float32"):
+        api.quantize_w4(np.ones((2, 64)), 32, dtype="float32")
