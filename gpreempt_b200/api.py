@@ -550,6 +550,7 @@ class FourBit:
 
     def free(self) -> None:
         self._buf.free()
+        self.struct.packed = None  # (products with weights that are gone are refused)
 
 
 def w4_matvec(w: FourBit, x, y, rows: int, ctx: LmContext, blp: BlpContext | None = None, stream=None, x_ld: int = 0, y_ld: int = 0) -> None:

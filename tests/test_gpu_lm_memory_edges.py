@@ -262,3 +262,15 @@ def test_batches_of_accounts_that_shared_memory_does_not_hold(gpx, ctx, kind, ke
         assert np.array_equal(got[s, :, :n], want) and np.all(got[s, :, n:] == -3), s
     assert ctx.status() == (0, 0)
     free(dw, ds, kept, counts, *arrays)
+
+
+def test_products_with_weights_that_are_gone_are_refused(gpx, ctx):
+    codes, scales, zeros = (up(gpx, a) for a in (np.zeros((16, 32), np.uint8), np.zeros((16, 1), np.uint16), np.zeros((16, 1), np.uint8)))
+    w, x, y = gpx.FourBit(codes, scales, zeros, 16, 64, 64, "bfloat16"), gpx.DeviceBuffer(128), gpx.DeviceBuffer(32)
+    gpx.w4_matvec(w, x, y, 1, ctx)
+    gpx.device_sync()
+    w.free()
+    with pytest.raises(Exception, match="packed"):
+        gpx.w4_matvec(w, x, y, 1, ctx)
+    w.free()
+    free(codes, scales, zeros, x, y)

@@ -301,3 +301,17 @@ def test_weights_without_a_scale_are_refused():
             api.quantize_w4(w, 32, dtype=dtype)
     with pytest.raises(ValueError, match="float32"):
         api.quantize_w4(np.ones((2, 64)), 32, dtype="float32")
+
+
+def test_weights_that_are_gone_have_no_address(lib):
+    """Products with them are refused, not run over memory that may be anybody's."""
+    from gpreempt_b200 import api
+
+    w = api.FourBit.__new__(api.FourBit)
+    w.struct = B.W4(P, 16, 64, 64, 1, b"bfloat16")
+    w._ref, w._buf = ctypes.byref(w.struct), api.DeviceBuffer.__new__(api.DeviceBuffer)
+    w._buf.ptr = ctypes.c_void_p()  # (no device memory here)
+    w.free()
+    assert w.struct.packed is None
+    a = B.W4MatvecArgs(x=P, y=P, rows=1)
+    refused(lib, B.FAIL, "packed", lib.gpx_w4_matvec(w._ref, ctypes.byref(a), ctypes.c_void_p(P), None, None))
