@@ -16,7 +16,7 @@ struct ChooseParams {
     const int *context;
     int *kept, *counts;
     long long kept_ld;
-    int seqs, keep, first, last;
+    int keep, first, last;
     int chunk;  // weights that shared memory has room for
     int *error;
 };
@@ -37,7 +37,7 @@ __device__ __forceinline__ unsigned rank_of(float w) {
 // writes it behind what the warps before it keep.
 //
 // The ranks of up to 16 384 tokens (32 768 with 1 024 threads) stay in shared memory, 32 a thread, a warp's in one stretch; longer
-// accounts are read again for every pass.  What bounds it is instructions, 70 % of the slots: 64 sequences of up to 16 384 tokens, 8 heads, 2 048 of them kept, 25.6 us (21 MB,
+// accounts are read again for every pass.  What bounds it is instructions, 70 % of the slots: 64 sequences of up to 16 384 tokens, 8 heads, 2 048 of them kept, 26.6 us (21 MB,
 // 0.8 TB/s); with every pass reading memory 57, with one load at a time 46, with a place for each ballot 48.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1)
@@ -443,7 +443,7 @@ int gpx_kv_choose(const gpx_kv_batch *batch, const gpx_kv_weights *account, cons
     GPX_REQUIRE((long long)b.seqs * p.account.kv_heads <= 0x7fffffff, GPX_OUT_OF_RANGE, "too many heads");
     const DeviceInfo &d = device_info();
     GPX_REQUIRE(d.device >= 0, GPX_FAIL, "gpx_init was not called");
-    p.context = b.context, p.seqs = b.seqs, p.kept = (int *)a.kept, p.counts = (int *)a.counts;
+    p.context = b.context, p.kept = (int *)a.kept, p.counts = (int *)a.counts;
     p.keep = a.keep, p.first = a.first, p.last = a.last, p.error = lm_ctx(ctx).error;
     blp_args.total_tiles = b.seqs * p.account.kv_heads;
     auto launch = [&](auto kernel, int threads) {
@@ -457,7 +457,9 @@ int gpx_kv_choose(const gpx_kv_batch *batch, const gpx_kv_weights *account, cons
         return launch_layer(kernel, grid, threads, smem, as_stream(stream), p, blp_args);
     };
     // Accounts that may be long and do not fill the SMs anyway have twice as many threads each.  With 1 024 and with 512, 8 heads: 16
-    // sequences of up to 32 000 tokens 19.1 and 38.7 us, 4 of up to 40 000 38.8 and 48.8, one of 131 072 100 and 136.
+    // sequences of up to 32 000 tokens 19.1 and 38.7 us, 4 of up to 40 000 38.8 and 48.8, one of 131 072 100 and 136.  (The host knows what
+    // accounts have room for, not how long they are: short ones in long accounts take 0.7 us more, 5.9 and 5.2 for one of 517 tokens, 8.3 and 7.6
+    // for 16 of 4 000; 16 of 12 000 take 11.5 and 12.3.)
     const bool wide = p.account.ld > 512 * kChooseHeld && blp_args.total_tiles <= d.sm_count;
     GPX_CUDA(wide ? launch(kv_choose_kernel<1024>, 1024) : launch(kv_choose_kernel<512>, 512));
     return GPX_SUCC;

@@ -3,15 +3,17 @@
 //   w_j = decay w_j (0 for a key of this step) + sum over rows r that see j of e^(scale q_r . k_j k_scale(page of j) - lse_r)
 //
 // The normalisers are known, so that keys need no look at one another: a key is read once, multiplied by all rows, and its row of
-// exponentials summed.  Bound by memory for few rows (D bytes of codes a key and head, 4 read and 4 written of its account, against
-// 2 D operations a row).  As in the attention of few rows, keys are the M side of the tensor instructions and rows the N side,
+// exponentials summed.  The floor is memory for few rows (D bytes of codes a key and head, 4 read and 4 written of its account, against
+// 2 D operations a row); from some eight rows on it is instructions, which for 64 rows, where keys are read twice, take five times as long
+// (the table below).  As in the attention of few rows, keys are the M side of the tensor instructions and rows the N side,
 // codes become halves in registers, and queries are halves of their row's power of two.  Nothing is shared between warps but the
 // queries, and codes go from memory to the registers where they are operands: a lane's elements of a key are 16-byte pieces.
 //
 // A warp takes sixteen keys of a block of 64; the sum over a key's rows stays in one warp, in the order of the rows, so that the
-// result does not depend on the launch.  Rows beyond what an instance holds go over the keys again.
+// result does not depend on the launch.  Rows beyond what an instance holds go over the keys again; the page of a key that any row
+// sees is looked up by every pass, so that all agree which keys have none.
 //
-// Measured, 32 heads of 128 on 8, bf16: single tokens of 64 sequences over 16 384 keys at most 126 us (608 MB, 4.8 TB/s; 116 where a part of
+// Measured, 32 heads of 128 on 8, bf16: single tokens of 64 sequences over 16 384 keys at most 125 us (608 MB, 4.9 TB/s; 116 where a part of
 // the keys is in L2 already), of one over 517 a launch.  238 instructions for sixteen keys and eight rows (their codes' conversions are
 // 32, the products 8) fill 56 % of the slots with 16 warps an SM: dependent ones, which more warps do not have registers to hide (five
 // CTAs an SM, at 96 registers, took 138 us, three, at 168, 138 too, with the operands of the rows in registers 120 against 119).
@@ -79,7 +81,8 @@ kv_weigh_kernel(const __grid_constant__ WeighParams p, BlpArgs blp) {
             const int slot = p.account.slots ? p.account.slots[s] : s;
             float *const account = p.account.weights + ((long long)slot * p.kv_heads + head) * p.account.ld;
             const int fresh = p.causal ? max(0, context - n) : context;  // keys from here on begin their account
-            const int seen = p.window && context - votes >= p.window ? context - votes - p.window + 1 : 0;  // the first key that a row sees (and those up to the last one are seen)
+            // the first key that a row sees (from there on some row sees each)
+            const int seen = p.window && context - votes >= p.window ? context - votes - p.window + 1 : 0;
             for (int row0 = 0; row0 < rows; row0 += ROWS) {
                 const int some_rows = min(ROWS, rows - row0);
                 auto position = [&](int r) { return context - votes + (row0 + r) / group; };  // (of the rows r of this pass)

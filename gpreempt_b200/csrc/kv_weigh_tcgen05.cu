@@ -9,7 +9,7 @@
 //
 // What should bound it is the special-function unit, sixteen exponentials a cycle and SM: 512 cycles a chunk, against 128 of the products.
 // A chunk takes 1 100 cycles an SM, with two warps of keys and two of rows on a scheduler, and the start and end of a tile 5 us, of which
-// the other CTA hides a part.  Four prompts' last 256 of 1 024 tokens over 8 192 keys at most, 32 heads of 128 on 8: 121 us (340 TFLOP/s, 1.3
+// the other CTA hides a part.  Four prompts' last 256 of 1 024 tokens over 8 192 keys at most, 32 heads of 128 on 8: 119 us (345 TFLOP/s, 1.3
 // T exponentials/s), 324 with the kernel for few rows.  Taken back: queries turned into halves by every tile, 495 us; one CTA an SM, 184;
 // chunks of 128 rows in two buffers, 132, and 74 us instead of 54 for tiles of one chunk.
 //

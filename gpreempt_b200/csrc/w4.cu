@@ -2,9 +2,11 @@
 //
 //   y[r][i] = sum over groups of scale[i][group] * (sum over j in it of (code[i][j] - zero[i][group]) x[r][j])
 //
-// Bound by memory: half a byte a weight, read once, against 2 operations a row.  Weights are the M side of the tensor instructions
-// (sixteen of their rows), the rows of x the N side.  A code becomes a 16-bit number without a conversion: or-ed into the mantissa
-// of 1024 (fp16) or 128 (bf16) it is that much more, and taking off that and the zero is exact.  Products of a group (64 elements at
+// The floor is memory: half a byte a weight, read once, against 2 operations a row; what bounds the kernels is their instructions (below).
+// Weights are the M side of the tensor instructions (sixteen of their rows), the rows of x the N side; 33 to 64 rows are two groups, for
+// which weights are read and converted twice.  A code becomes a 16-bit number without a conversion: or-ed into the mantissa
+// of 1024 (fp16) or 128 (bf16) it is that much more, and taking off that and the zero is exact (the method of Kim, Henry, Fahim and
+// Hassan Awadalla, 2022).  Products of a group (64 elements at
 // most) are summed in float and then multiplied by the scale in float, so that nothing is rounded but the sums.  (Leaving the zeros to
 // the sums of x instead saves sixteen subtractions for 512 bytes of weights, and costs as many instructions behind the products.)
 //
@@ -26,35 +28,38 @@ constexpr int kW4Sets = kW4Elements / G;         // scales of a row in a record:
 
 struct W4Params {
     const unsigned char *packed;
-    int n, k, tiles16, blocks, records;  // tiles of sixteen rows; blocks and records of a row
+    int n, k, tiles16, records;          // tiles of sixteen rows; records of a row
     int record_bytes, zeros;
     const unsigned short *x;
     unsigned short *y;
     long long x_ld, y_ld;
     int rows;
     int row_groups, group_rows;          // rows of x that are multiplied at a time
-    int row_tiles, steps, line;          // tiles of 512 rows of weights, steps of 128 elements of a row, steps of everything
+    int row_tiles, steps, line;          // tiles of 256 rows of weights, steps of 128 elements of a row, steps of everything
     int steps_a_tile, most_tiles;
     int *counters;
     float *slots;
 };
 
 // Bytes of weights from which the kernel of large products takes over.  Both, us, in bf16 groups of 128:
-//   rows            4096 x 4096   8192 x 4096   14336 x 4096   8192 x 8192   28672 x 8192
-//      1   small          7.2          13.1           17.0          21.0           45
-//          large         11.1          12.2           14.9          17.1           37
-//     24   small         14.5          23.9           37.5          41.1          120
-//          large         17.4          18.9           23.5          25.9           60
+//   rows            4096 x 4096   8192 x 4096   14336 x 4096   8192 x 8192   28672 x 8192   1024 x 16384
+//      1   small          7.0          11.4           15.7          18.7           42             16.0
+//          large         10.9          12.2           15.0          16.7           37             20.5
+//     24   small         12.5          21.6           35.0          36.6          114             16.6
+//          large         16.6          18.3           22.7          25.1           58             31.7
+//     64   small         27            50             85            86            287             30.9
+//          large         20            27             39            42            118             30.9
+// (4096 x 4096, 8.9 MB, stays with the small one, which is the slower from 40 rows on)
 constexpr long long kW4Large = 12 << 20;
 constexpr uint32_t kW4HalfBase = 0x6400, kW4BfBase = 0x4300;  // 1024 in fp16, 128 in bf16: a code is or-ed into the mantissa
 
 struct W4Layout {
-    int tiles16, blocks, records, record_bytes;
+    int tiles16, records, record_bytes;
     size_t bytes;
 };
 static W4Layout w4_layout(const gpx_w4 &w) {
     W4Layout l;
-    l.tiles16 = (w.n + 15) / 16, l.blocks = (w.k + 63) / 64, l.records = (l.blocks + kW4Blocks - 1) / kW4Blocks;
+    l.tiles16 = (w.n + 15) / 16, l.records = (w.k + kW4Elements - 1) / kW4Elements;
     l.record_bytes = kW4Codes + kW4Elements / w.group * 32 * (w.zeros ? 2 : 1);
     l.bytes = ((size_t)l.tiles16 * l.records * l.record_bytes + 255) / 256 * 256;
     return l;
@@ -68,6 +73,7 @@ __device__ __forceinline__ uint32_t w4_order(uint32_t w) {
     return to;
 }
 
+// Once a matrix; of 28 672 x 8 192 elements with zeros, groups of 64, 93 us, of 4 096 x 4 096 10.
 __global__ void w4_pack_kernel(const unsigned char *codes, const unsigned short *scales, const unsigned char *zeros, int n, int k, int group, int tiles16,
                                int records, bool half, unsigned char *packed) {
     pdl_enter();
@@ -401,7 +407,7 @@ w4_stream_kernel(const __grid_constant__ W4Params p, BlpArgs blp) {
         int slot = 0;
 
         for (int begin = line0; begin < line1;) {
-            // ---- steps [begin, end) of one tile of 512 rows of weights and a group of rows of x
+            // ---- steps [begin, end) of one tile of 256 rows of weights and a group of rows of x
             const int unit0 = begin - now.step, end = min(line1, unit0 + p.steps);
             const int first_row = now.row_group * p.group_rows, rows = min(p.group_rows, p.rows - first_row);
             const int tile16 = (now.row_tile * kW4StreamWarps + wid) * 2;
@@ -591,7 +597,7 @@ int gpx_w4_matvec(const gpx_w4 *w, const gpx_w4_matvec_args *args, void *ctx, co
     GPX_REQUIRE(d.device >= 0, GPX_FAIL, "gpx_init was not called");
     const W4Layout l = w4_layout(*w);
     p.packed = (const unsigned char *)w->packed, p.record_bytes = l.record_bytes, p.zeros = w->zeros != 0;
-    p.n = w->n, p.k = w->k, p.tiles16 = l.tiles16, p.blocks = l.blocks, p.records = l.records;
+    p.n = w->n, p.k = w->k, p.tiles16 = l.tiles16, p.records = l.records;
     p.x = (const unsigned short *)a.x, p.y = (unsigned short *)a.y, p.rows = a.rows;
     const LmCtx c = lm_ctx(ctx);
     p.counters = c.counters, p.slots = c.parts;

@@ -77,7 +77,7 @@ def _bf16(x: np.ndarray) -> np.ndarray:
 class Decoder:
     """Weights, cache and buffers of a tenant; `word` makes its launches preemptible.  With `keep` a conversation of 2 x keep tokens and
     more keeps that many behind a step, and `room` is how many it may hold at once (0: most_tokens; not below 2 x keep, where it would never
-    drop any); with `four_bit` steps of a few tokens read weights of 4 bits."""
+    drop any); a `window` is then that many kept tokens.  With `four_bit` steps of up to 64 tokens read weights of 4 bits."""
 
     HEADS, KV_HEADS, DIM, PAGE, VOCAB, TILE = 8, 2, 64, 32, 4096, 128
     GROUP, FIRST = 64, 4  # elements that have one scale; tokens at the start of a conversation that it always keeps
@@ -154,6 +154,7 @@ class Decoder:
         return packed
 
     def _gemm(self, which: int, a, b, c, rows: int, n: int) -> None:
+        # (these weights, 5.1 us with 4 bits and 10.5 with 16 for 512 x 512, 10.4 both for 64 rows by 4 096 x 512)
         if self.w4 and rows <= 64:
             self._run(lambda: api.w4_matvec(self.w4[which], a, c, rows, self.ctx, self.blp, self.stream))
             return

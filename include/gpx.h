@@ -374,9 +374,11 @@ typedef struct gpx_kv_weights {
  * heads, causal, window, scale and dtype are what gpx_kv_attend took, lse [token][heads] what it left.  Without `causal` the new
  * tokens are not among the keys, and every account goes on.  Sequences without new tokens keep their accounts as they are, and so
  * do keys that some of these rows see and whose page is outside the cache (code 2); pages of keys that none sees are not looked
- * up.  decay is above 0 and at most 1.  Sums are float, in an order that does not depend on the launch; queries as products see
- * them are those of gpx_kv_attend.  A key whose score is not a number for a row that sees it has an account that is not a
- * number; rows that do not see it have no influence. */
+ * up.  `window` counts places in the cache, as in gpx_kv_attend: behind an eviction these are kept tokens, which may reach much
+ * farther back than as many positions.  decay is above 0 and at most 1.  Sums are float, in an order that does not depend on the
+ * launch.  Up to 64 rows a head of keys (heads / kv_heads x the most tokens of a sequence that count) queries as products see them are those of
+ * gpx_kv_attend; more are multiplied as they are, also in bfloat16.  A key whose score is not a number for a row that sees it has an
+ * account that is not a number; rows that do not see it have no influence. */
 typedef struct gpx_kv_weigh_args {
     const void *q, *lse;
     long long q_ld;
@@ -427,7 +429,8 @@ int gpx_w4_bytes(const gpx_w4 *w, size_t *bytes);
 int gpx_w4_pack(const gpx_w4 *w, const void *codes, const void *scales, const void *zeros, gpx_stream s);
 /* y[r][i] = sum over j of x[r][j] w[i][j] for 1 to 64 rows; x and y have the weights' dtype, x_ld and y_ld elements from one
  * row to the next (0: packed; x 16-byte aligned, x_ld a multiple of 8).  Products of codes and x are exact, sums float; a result is
- * rounded once. */
+ * rounded once.  The scale of a group multiplies its sum: of bfloat16 rows of 2^118 and more the sum of a group may leave the range of float
+ * where the scaled products would not. */
 typedef struct gpx_w4_matvec_args {
     const void *x;
     void *y;
