@@ -208,3 +208,23 @@ def test_append_at_stops_between_tiles(gpx, ctx):
                                                            ctx, rope, where, blp, s, width, width, width),
                  lambda: [q.download(np.uint16), *bed.download()], fresh, 120)
     free(x, q, dcos, dsin, dat, bed)
+
+
+@pytest.mark.parametrize("new,most", [(1, 30000), (4, 20000)])
+def test_attention_of_few_rows_leaves_nothing_in_the_context(gpx, ctx, new, most):
+    heads, kv, dim, page, seqs = 16, 4, 128, 64, 12
+    bed = Bed(gpx, [new] * seqs, [most - 501 * i for i in range(seqs)], heads, kv, dim, page, seed=4).upload()
+    dq = up(gpx, to_bits(bed.rng.standard_normal((bed.tokens, heads, dim)), "bfloat16"))
+    out = gpx.DeviceBuffer(dq.nbytes)
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.kv_attend(bed.cache, bed.batch, dq, out, heads, "bfloat16", ctx, blp=blp, stream=s),
+                 lambda: [out.download(np.uint16)], out.zero, 100)
+    free(dq, out, bed)
+
+
+def test_scores_leave_nothing_in_the_context(gpx, ctx):
+    rows, vocab = 4000, 20000
+    x = up(gpx, to_bits(np.random.default_rng(1).standard_normal((rows, vocab)) * 4, "float16"))
+    entropy, ids = gpx.DeviceBuffer(rows * 4), gpx.DeviceBuffer(rows * 4)
+    stopped_runs(gpx, ctx, lambda blp, s: gpx.token_scores(x, rows, vocab, "float16", ctx, None, None, entropy, top=1, top_ids=ids, blp=blp, stream=s),
+                 lambda: [entropy.download(np.float32), ids.download(np.int32)], lambda: (entropy.zero(), ids.zero()), 60)
+    free(x, entropy, ids)
